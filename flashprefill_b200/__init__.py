@@ -8,13 +8,16 @@ A caller written against the reference's ``ops`` package can call ``install_as_o
 once; ``import ops`` then resolves to this package.
 """
 from ._lib import FlashPrefillError
-from ._ops import check_device_error, get_mean_warps, search_dense, search_varlen, set_mean_warps
+from ._ops import (check_device_error, check_paged_error, get_mean_warps, paged_decode_workspace_bytes, search_dense,
+                   search_varlen, set_mean_warps)
 from .flashprefill_native_forward import flash_prefill
 from .flashprefill_varlen_func import flash_prefill_varlen_func
+from .paged_cache import KVCache, kv_cache_alloc, kv_cache_read, kv_cache_write, paged_decode
 from . import torch_ops  # registers torch.ops.flashprefill.prefill_dense / prefill_varlen
 
 __all__ = ["flash_prefill", "flash_prefill_varlen_func", "search_dense", "search_varlen", "set_mean_warps",
-           "get_mean_warps", "check_device_error", "FlashPrefillError", "install_as_ops"]
+           "get_mean_warps", "check_device_error", "FlashPrefillError", "install_as_ops", "KVCache", "kv_cache_alloc",
+           "kv_cache_write", "kv_cache_read", "paged_decode", "paged_decode_workspace_bytes", "check_paged_error"]
 
 
 def install_as_ops() -> None:

@@ -14,19 +14,22 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FLASHPREFILL_B200_LIB") or os.path.join(_HERE, "libflashprefill_b200.so")
 
 FPB_OK, FPB_EINVAL, FPB_ECUDA, FPB_EDEVICE = 0, 1, 2, 3
-FPB_BF16, FPB_FP16 = 0, 1
+FPB_BF16, FPB_FP16, FPB_E4M3 = 0, 1, 2
 
 DEV_ERROR_BITS = {
     1: "pipeline wait timed out",
     2: "cu_seqlens not non-decreasing from 0 to total_tokens",
     4: "a sequence is longer than max_seq_len",
     8: "a block list held an index outside [0, query block]",
+    16: "a slot or page-table entry outside the paged cache",
+    32: "a sequence length outside [0, room of its pages or output]",
 }
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_I64 = ctypes.c_int64
 _I64P = ctypes.POINTER(ctypes.c_int64)
 _U32P = ctypes.POINTER(ctypes.c_uint32)
 
@@ -60,6 +63,14 @@ SIGNATURES = {
     "fpb_test_set_fault": (_I, [_I, ctypes.c_ulonglong]),
     "fpb_prefill_dense_noalloc": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I64P, _I64P, _I64P, _I64P,
                                        _I, _I, _I, _F, _I, _I, _I, _P]),
+    "fpb_kv_cache_write": (_I, [_P, _P, _I, _I, _I, _I, _I64P, _I64P, _P, _P, _I, _I, _I, _I64P, _P, _P, _I64P, _P, _I,
+                                _P]),
+    "fpb_kv_cache_read": (_I, [_P, _P, _I, _I, _I, _I, _I, _I64P, _P, _P, _I64P, _P, _I64, _I, _P, _I, _P, _P, _I, _I,
+                               _I64P, _I64P, _P]),
+    "fpb_paged_decode_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "fpb_paged_decode": (_I, [_P, _I, _I, _I, _I, _I, _I64P, _P, _P, _I, _I, _I, _I64P, _P, _P, _I64P, _P, _I64, _I, _P,
+                              _P, _I64P, _P, _F, _P, _SZ, _P]),
+    "fpb_paged_read_device_error": (_I, [_U32P, _P]),
 }
 
 _lock = threading.Lock()

@@ -19,6 +19,8 @@
 #include "fp_attn.cu"
 #include "fp_attn2.cu"
 #include "fp_mean.cu"
+#include "fp_paged.cu"
+#include "fp_decode.cu"
 #include "fp_search.cu"
 
 namespace fpb {
@@ -901,3 +903,4 @@ int fpb_read_device_error(const void* workspace, uint32_t* flags, void* stream) 
 }  // extern "C"
 
 #include "fp_noalloc.cu"
+#include "fp_paged_api.cu"

@@ -1,0 +1,274 @@
+// C ABI of the paged cache (fp_paged.cu) and of decode attention over it (fp_decode.cu).  Included at the end of fp_api.cu
+// (one translation unit): argument checks and launches.
+namespace fpb {
+namespace {
+
+// The cache arguments shared by the three entry points.  out: C with byte strides.
+int make_cache(PagedCache* C, const void* k_cache, const void* v_cache, int cache_dtype, int dtype, int num_pages,
+               int page_size, int hk, int head_dim, const int64_t* cs, const float* k_scale, const float* v_scale,
+               const int64_t* ss) {
+  FPB_CHECK_ARG(dtype == FPB_BF16 || dtype == FPB_FP16, "dtype must be FPB_BF16 or FPB_FP16 (got %d)", dtype);
+  FPB_CHECK_ARG(cache_dtype == dtype || cache_dtype == FPB_E4M3,
+                "the cache must hold the rows' 16-bit type or FPB_E4M3 (got %d for rows of %d)", cache_dtype, dtype);
+  FPB_CHECK_ARG(head_dim == kHeadDim, "head_dim must be 128 (got %d)", head_dim);
+  FPB_CHECK_ARG(num_pages >= 1 && page_size >= 1 && hk >= 1, "num_pages (%d), page_size (%d) and num_kv_heads (%d) must be >= 1",
+                num_pages, page_size, hk);
+  FPB_TRY(check_ptr(k_cache, "k_cache"));
+  FPB_TRY(check_ptr(v_cache, "v_cache"));
+  const int elt = cache_dtype == FPB_E4M3 ? 1 : 2;
+  FPB_CHECK_ARG(cs != nullptr, "cache strides are NULL");
+  for (int i = 0; i < 3; ++i) {
+    FPB_CHECK_ARG(cs[i] >= 0 && cs[i] * elt % 16 == 0, "cache stride[%d]=%lld must be a non-negative multiple of 16 bytes", i,
+                  (long long)cs[i]);
+    FPB_CHECK_ARG(cs[i] < (int64_t(1) << 40), "cache stride[%d] too large", i);
+  }
+  C->k = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+  C->v = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  C->s_page = cs[0] * elt;
+  C->s_tok = cs[1] * elt;
+  C->s_head = cs[2] * elt;
+  C->num_pages = num_pages;
+  C->page_size = page_size;
+  C->k_scale = C->v_scale = nullptr;
+  C->ss_page = C->ss_tok = C->ss_head = 0;
+  if (cache_dtype == FPB_E4M3) {
+    FPB_CHECK_ARG(k_scale != nullptr && v_scale != nullptr, "an e4m3 cache needs k_scale and v_scale");
+    FPB_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) & 3) == 0,
+                  "k_scale and v_scale must be aligned float pointers");
+    FPB_CHECK_ARG(ss != nullptr, "scale strides are NULL");
+    for (int i = 0; i < 3; ++i)
+      FPB_CHECK_ARG(ss[i] >= 0 && ss[i] < (int64_t(1) << 40), "scale stride[%d]=%lld is out of range", i, (long long)ss[i]);
+    C->k_scale = const_cast<float*>(k_scale);
+    C->v_scale = const_cast<float*>(v_scale);
+    C->ss_page = ss[0];
+    C->ss_tok = ss[1];
+    C->ss_head = ss[2];
+  } else {
+    FPB_CHECK_ARG(k_scale == nullptr && v_scale == nullptr, "a 16-bit cache takes no scales");
+  }
+  return FPB_OK;
+}
+
+int check_table(const int32_t* table, int64_t stride, int max_pages, int page_size, const int32_t* seq_lens, int batch) {
+  FPB_CHECK_ARG(batch >= 1 && max_pages >= 1, "batch (%d) and max_pages (%d) must be >= 1", batch, max_pages);
+  FPB_CHECK_ARG((int64_t)max_pages * page_size <= kPagedMaxLen, "max_pages * page_size must be at most %lld",
+                (long long)kPagedMaxLen);
+  FPB_CHECK_ARG(table != nullptr && (reinterpret_cast<uintptr_t>(table) & 3) == 0, "page_table must be an aligned int32 pointer");
+  FPB_CHECK_ARG(seq_lens != nullptr && (reinterpret_cast<uintptr_t>(seq_lens) & 3) == 0,
+                "seq_lens must be an aligned int32 pointer");
+  FPB_CHECK_ARG(stride >= 0 && stride < (int64_t(1) << 40), "page_table stride %lld is out of range", (long long)stride);
+  return FPB_OK;
+}
+
+// How the query heads of a KV head become items: equal groups of at most 16.
+void head_groups(int G, int* ngroups, int* nh) {
+  const int n = (G + 15) / 16;
+  *nh = (G + n - 1) / n;
+  *ngroups = (G + *nh - 1) / *nh;
+}
+
+// Units that an item can have, and the CTAs that can have work.
+struct DecodeShape {
+  int G, ngroups, nh, unit, max_ctas;
+  bool split;
+};
+DecodeShape decode_shape(int batch, int hq, int hk, int cache_dtype, int max_pages, int page_size) {
+  DecodeShape s{};
+  s.G = hq / hk;
+  head_groups(s.G, &s.ngroups, &s.nh);
+  s.unit = kDecWarps * (cache_dtype == FPB_E4M3 ? 32 : 16);
+  const int64_t units = ((int64_t)max_pages * page_size + s.unit - 1) / s.unit;
+  s.split = units > 1;
+  const int64_t items = (int64_t)batch * hk * s.ngroups;
+  s.max_ctas = (int)std::min<int64_t>(kDecMaxCtas, units >= kDecMaxCtas ? kDecMaxCtas : items * units);
+  return s;
+}
+int64_t decode_ws_part(const DecodeShape& s) { return align256(16 * (int64_t)s.max_ctas); }
+int64_t decode_ws_ml(const DecodeShape& s) {
+  return decode_ws_part(s) + align256(2 * (int64_t)s.max_ctas * s.nh * kHeadDim * 4);
+}
+int64_t decode_ws_total(const DecodeShape& s) {
+  return s.split ? decode_ws_ml(s) + align256(2 * (int64_t)s.max_ctas * s.nh * 8) : 0;
+}
+
+template <typename T, bool kE4m3, int NT>
+int launch_decode(const DecodeArgs& A, int ctas, bool split, cudaStream_t stream) {
+  auto kernel = paged_decode_kernel<T, kE4m3, NT>;
+  FPB_TRY(set_smem(kernel, kDecSmemBytes));
+  kernel<<<ctas, kDecThreads, kDecSmemBytes, stream>>>(A);
+  FPB_CUDA(cudaGetLastError());
+  if (!split) return FPB_OK;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FPB_CUDA(cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<T>, A));
+  return FPB_OK;
+}
+
+}  // namespace
+}  // namespace fpb
+
+extern "C" {
+
+int fpb_kv_cache_write(const void* k, const void* v, int dtype, int tokens, int hk, int head_dim, const int64_t* k_strides,
+                       const int64_t* v_strides, void* k_cache, void* v_cache, int cache_dtype, int num_pages, int page_size,
+                       const int64_t* cache_strides, float* k_scale, float* v_scale, const int64_t* scale_strides,
+                       const void* slots, int slot_bytes, void* stream) {
+  KvWriteArgs A{};
+  FPB_TRY(make_cache(&A.C, k_cache, v_cache, cache_dtype, dtype, num_pages, page_size, hk, head_dim, cache_strides, k_scale,
+                     v_scale, scale_strides));
+  FPB_CHECK_ARG(tokens >= 0, "tokens (%d) must be >= 0", tokens);
+  FPB_CHECK_ARG((int64_t)tokens * hk < (int64_t(1) << 31), "tokens * num_kv_heads must be below 2^31");
+  FPB_CHECK_ARG(slot_bytes == 4 || slot_bytes == 8, "slot_bytes must be 4 or 8 (got %d)", slot_bytes);
+  if (tokens == 0) return FPB_OK;
+  FPB_TRY(check_ptr(k, "k"));
+  FPB_TRY(check_ptr(v, "v"));
+  FPB_TRY(check_strides(k_strides, 2, "k"));
+  FPB_TRY(check_strides(v_strides, 2, "v"));
+  FPB_CHECK_ARG(slots != nullptr && reinterpret_cast<uintptr_t>(slots) % slot_bytes == 0, "slots must be an aligned pointer");
+  A.k = static_cast<const uint8_t*>(k);
+  A.v = static_cast<const uint8_t*>(v);
+  A.ks_tok = 2 * k_strides[0];
+  A.ks_head = 2 * k_strides[1];
+  A.vs_tok = 2 * v_strides[0];
+  A.vs_head = 2 * v_strides[1];
+  A.slots = slots;
+  A.slots64 = slot_bytes == 8;
+  A.rows = (unsigned)tokens * (unsigned)hk;
+  A.hk = hk;
+  auto st = static_cast<cudaStream_t>(stream);
+  if (cache_dtype != FPB_E4M3) kv_write_copy_kernel<<<(A.rows + 15) / 16, 256, 0, st>>>(A);
+  else if (dtype == FPB_BF16) kv_write_e4m3_kernel<__nv_bfloat16><<<(A.rows + 31) / 32, 256, 0, st>>>(A);
+  else kv_write_e4m3_kernel<__half><<<(A.rows + 31) / 32, 256, 0, st>>>(A);
+  FPB_CUDA(cudaGetLastError());
+  return FPB_OK;
+}
+
+int fpb_kv_cache_read(const void* k_cache, const void* v_cache, int cache_dtype, int num_pages, int page_size, int hk,
+                      int head_dim, const int64_t* cache_strides, const float* k_scale, const float* v_scale,
+                      const int64_t* scale_strides, const int32_t* page_table, int64_t table_stride, int max_pages,
+                      const int32_t* seq_lens, int batch, void* k, void* v, int dtype, int out_len, const int64_t* k_strides,
+                      const int64_t* v_strides, void* stream) {
+  KvReadArgs A{};
+  FPB_TRY(make_cache(&A.C, k_cache, v_cache, cache_dtype, dtype, num_pages, page_size, hk, head_dim, cache_strides, k_scale,
+                     v_scale, scale_strides));
+  FPB_TRY(check_table(page_table, table_stride, max_pages, page_size, seq_lens, batch));
+  FPB_CHECK_ARG(batch <= 65535, "batch (%d) must be at most 65535", batch);
+  FPB_CHECK_ARG(out_len >= 1 && (int64_t)out_len * hk < (int64_t(1) << 31), "out_len (%d) must be >= 1 and out_len * num_kv_heads below 2^31",
+                out_len);
+  FPB_TRY(check_ptr(k, "k"));
+  FPB_TRY(check_ptr(v, "v"));
+  FPB_TRY(check_strides(k_strides, 3, "k"));
+  FPB_TRY(check_strides(v_strides, 3, "v"));
+  A.page_table = page_table;
+  A.table_stride = table_stride;
+  A.max_pages = max_pages;
+  A.seq_lens = seq_lens;
+  A.out_len = out_len;
+  A.hk = hk;
+  A.k = static_cast<uint8_t*>(k);
+  A.v = static_cast<uint8_t*>(v);
+  A.ks_b = 2 * k_strides[0];
+  A.ks_tok = 2 * k_strides[1];
+  A.ks_head = 2 * k_strides[2];
+  A.vs_b = 2 * v_strides[0];
+  A.vs_tok = 2 * v_strides[1];
+  A.vs_head = 2 * v_strides[2];
+  const unsigned rows = (unsigned)out_len * (unsigned)hk;
+  auto st = static_cast<cudaStream_t>(stream);
+  if (cache_dtype != FPB_E4M3) kv_read_copy_kernel<<<dim3((rows + 15) / 16, batch), 256, 0, st>>>(A);
+  else if (dtype == FPB_BF16) kv_read_e4m3_kernel<__nv_bfloat16><<<dim3((rows + 31) / 32, batch), 256, 0, st>>>(A);
+  else kv_read_e4m3_kernel<__half><<<dim3((rows + 31) / 32, batch), 256, 0, st>>>(A);
+  FPB_CUDA(cudaGetLastError());
+  return FPB_OK;
+}
+
+size_t fpb_paged_decode_workspace_bytes(int batch, int hq, int hk, int cache_dtype, int max_pages, int page_size) {
+  if (batch < 1 || hq < 1 || hk < 1 || hq % hk != 0 || max_pages < 1 || page_size < 1) return 0;
+  return (size_t)decode_ws_total(decode_shape(batch, hq, hk, cache_dtype, max_pages, page_size));
+}
+
+int fpb_paged_decode(const void* q, int dtype, int batch, int hq, int hk, int head_dim, const int64_t* q_strides,
+                     const void* k_cache, const void* v_cache, int cache_dtype, int num_pages, int page_size,
+                     const int64_t* cache_strides, const float* k_scale, const float* v_scale, const int64_t* scale_strides,
+                     const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* seq_lens, void* out,
+                     const int64_t* o_strides, float* lse, float sm_scale, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  DecodeArgs A{};
+  FPB_TRY(make_cache(&A.C, k_cache, v_cache, cache_dtype, dtype, num_pages, page_size, hk, head_dim, cache_strides, k_scale,
+                     v_scale, scale_strides));
+  FPB_CHECK_ARG(hq >= 1 && hq % hk == 0, "num_q_heads (%d) must be a multiple of num_kv_heads (%d)", hq, hk);
+  FPB_TRY(check_table(page_table, table_stride, max_pages, page_size, seq_lens, batch));
+  FPB_CHECK_ARG((int64_t)batch * hq < (int64_t(1) << 31), "batch * num_q_heads must be below 2^31");
+  FPB_TRY(check_ptr(q, "q"));
+  FPB_TRY(check_strides(q_strides, 2, "q"));
+  FPB_CHECK_ARG(out != nullptr && (reinterpret_cast<uintptr_t>(out) & 1) == 0, "out must be an aligned pointer");
+  FPB_CHECK_ARG(o_strides != nullptr, "out strides are NULL");
+  for (int i = 0; i < 2; ++i)
+    FPB_CHECK_ARG(o_strides[i] >= 0 && o_strides[i] < (int64_t(1) << 40), "out stride[%d]=%lld is out of range", i,
+                  (long long)o_strides[i]);
+  FPB_CHECK_ARG((reinterpret_cast<uintptr_t>(lse) & 3) == 0, "lse must be an aligned float pointer or NULL");
+  FPB_CHECK_ARG(std::isfinite(sm_scale), "sm_scale must be finite");
+  const DecodeShape s = decode_shape(batch, hq, hk, cache_dtype, max_pages, page_size);
+  if (s.split) {
+    FPB_CHECK_ARG(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
+                  "workspace must be a 256-byte aligned device pointer");
+    FPB_CHECK_ARG((int64_t)workspace_bytes >= decode_ws_total(s), "workspace too small: %zu bytes given, %lld needed",
+                  workspace_bytes, (long long)decode_ws_total(s));
+    auto* ws = static_cast<uint8_t*>(workspace);
+    A.desc = reinterpret_cast<int4*>(ws);
+    A.part = reinterpret_cast<float*>(ws + decode_ws_part(s));
+    A.ml = reinterpret_cast<float2*>(ws + decode_ws_ml(s));
+  }
+  A.q = static_cast<const uint8_t*>(q);
+  A.out = static_cast<uint8_t*>(out);
+  A.lse = lse;
+  A.q_b = 2 * q_strides[0];
+  A.q_h = 2 * q_strides[1];
+  A.o_b = 2 * o_strides[0];
+  A.o_h = 2 * o_strides[1];
+  A.page_table = page_table;
+  A.table_stride = table_stride;
+  A.seq_lens = seq_lens;
+  A.max_pages = max_pages;
+  A.batch = batch;
+  A.hq = hq;
+  A.hk = hk;
+  A.G = s.G;
+  A.ngroups = s.ngroups;
+  A.nh = s.nh;
+  A.c = (float)(sm_scale * 1.4426950408889634);
+  int sms = 0;
+  FPB_TRY(sm_count(&sms));
+  const int ctas = std::min(s.max_ctas, sms * kDecCtasPerSm);
+  auto st = static_cast<cudaStream_t>(stream);
+  const bool bf16 = dtype == FPB_BF16, e4m3 = cache_dtype == FPB_E4M3, wide = s.nh > 8;
+  if (bf16) {
+    if (e4m3) return wide ? launch_decode<__nv_bfloat16, true, 2>(A, ctas, s.split, st) : launch_decode<__nv_bfloat16, true, 1>(A, ctas, s.split, st);
+    return wide ? launch_decode<__nv_bfloat16, false, 2>(A, ctas, s.split, st) : launch_decode<__nv_bfloat16, false, 1>(A, ctas, s.split, st);
+  }
+  if (e4m3) return wide ? launch_decode<__half, true, 2>(A, ctas, s.split, st) : launch_decode<__half, true, 1>(A, ctas, s.split, st);
+  return wide ? launch_decode<__half, false, 2>(A, ctas, s.split, st) : launch_decode<__half, false, 1>(A, ctas, s.split, st);
+}
+
+int fpb_paged_read_device_error(uint32_t* flags, void* stream) {
+  FPB_CHECK_ARG(flags != nullptr, "flags is NULL");
+  auto st = static_cast<cudaStream_t>(stream);
+  uint32_t h = 0;
+  FPB_CUDA(cudaMemcpyFromSymbolAsync(&h, g_paged_err, sizeof(h), 0, cudaMemcpyDeviceToHost, st));
+  FPB_CUDA(cudaStreamSynchronize(st));
+  *flags = h;
+  if (h == 0) return FPB_OK;
+  paged_clear_err_kernel<<<1, 1, 0, st>>>(h);
+  FPB_CUDA(cudaGetLastError());
+  FPB_CUDA(cudaStreamSynchronize(st));
+  return fail(FPB_EDEVICE, "device error bits 0x%x", h);
+}
+
+}  // extern "C"

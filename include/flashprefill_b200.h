@@ -48,12 +48,15 @@ extern "C" {
 
 #define FPB_BF16 0
 #define FPB_FP16 1
+#define FPB_E4M3 2 /* paged caches only: 8-bit codes with a float scale for each (token, head) */
 
 /* Device error bits (fpb_read_device_error). */
 #define FPB_DEV_WAIT_TIMEOUT 1u   /* a pipeline wait ran out of time; the kernel bailed out */
 #define FPB_DEV_BAD_SEQLENS 2u    /* cu_seqlens not non-decreasing from 0 to total_tokens */
 #define FPB_DEV_SEQ_TOO_LONG 4u   /* a sequence longer than max_seq_len (rows skipped) */
 #define FPB_DEV_INDEX_RANGE 8u    /* a block list held an index outside [0, query block] */
+#define FPB_DEV_BAD_PAGE 16u      /* paged cache: a slot or page-table entry outside the cache (skipped) */
+#define FPB_DEV_BAD_LENGTH 32u    /* paged cache: a sequence length outside [0, room] */
 
 /* Library version (major*10000 + minor*100 + patch). */
 FPB_API int fpb_version(void);
@@ -217,6 +220,50 @@ FPB_API int fpb_test_set_fault(int withhold_first_load, unsigned long long wait_
  * returns FPB_EDEVICE if any bit is set.  No counterpart in the reference, which has no
  * device-side error reporting. */
 FPB_API int fpb_read_device_error(const void* workspace, uint32_t* flags, void* stream);
+
+/* ---- Paged key/value cache and decode attention (no counterpart in the reference, which leaves decode to its host
+ * framework).  A cache is (num_pages, page_size, hk, 128): k_cache and v_cache share cache_strides = {page, token, head}
+ * in ELEMENTS (multiples of 16 bytes; last dimension contiguous).  cache_dtype is the rows' dtype, or FPB_E4M3: codes with
+ * k_scale / v_scale, float (num_pages, page_size, hk) with scale_strides = {page, token, head} in elements; a value is
+ * code * scale.  16-bit caches take NULL scales.  page_table: int32 (batch, max_pages), row stride table_stride;
+ * seq_lens: int32 (batch).  Both live on the device and are checked there: an entry that points outside the cache, a slot
+ * beyond it or a length outside [0, room] sets an error bit of the current device, which stays until
+ * fpb_paged_read_device_error reads it; nothing outside the tensors is touched. */
+
+/* Rows k, v (tokens, hk, 128), strides {token, head}, into the cache slots slots[t] = page * page_size + offset (int32 or
+ * int64: slot_bytes 4 or 8).  A negative slot skips its row (padding).  Slots must differ from one another; where two rows
+ * name one slot, what it holds is not defined.  For FPB_E4M3 each row's scale is max(max|x|, 2^-100) / 448. */
+FPB_API int fpb_kv_cache_write(const void* k, const void* v, int dtype, int tokens, int hk, int head_dim,
+                               const int64_t* k_strides, const int64_t* v_strides, void* k_cache, void* v_cache,
+                               int cache_dtype, int num_pages, int page_size, const int64_t* cache_strides,
+                               float* k_scale, float* v_scale, const int64_t* scale_strides, const void* slots,
+                               int slot_bytes, void* stream);
+
+/* The first seq_lens[b] cached rows of every sequence into k, v (batch, out_len, hk, 128), strides {batch, token, head}.
+ * Later rows, and those of a sequence or page that is in error, are left as they were. */
+FPB_API int fpb_kv_cache_read(const void* k_cache, const void* v_cache, int cache_dtype, int num_pages, int page_size,
+                              int hk, int head_dim, const int64_t* cache_strides, const float* k_scale,
+                              const float* v_scale, const int64_t* scale_strides, const int32_t* page_table,
+                              int64_t table_stride, int max_pages, const int32_t* seq_lens, int batch, void* k, void* v,
+                              int dtype, int out_len, const int64_t* k_strides, const int64_t* v_strides, void* stream);
+
+/* Workspace of fpb_paged_decode (0 where none is needed: sequences of at most one unit of work). */
+FPB_API size_t fpb_paged_decode_workspace_bytes(int batch, int hq, int hk, int cache_dtype, int max_pages,
+                                                int page_size);
+
+/* Attention of one new token a sequence, q (batch, hq, 128), over its seq_lens[b] cached tokens (the new token's own row
+ * is written first, by fpb_kv_cache_write).  out like q, strides {batch, head}; lse: NULL or float (batch, hq) contiguous,
+ * the natural logarithm of the sum of exp(sm_scale q.k).  A sequence of length 0 (or in error) gives zeros and -inf; tokens
+ * of a page in error are left out.  The workspace needs no initialisation; calls that overlap on the GPU need one each. */
+FPB_API int fpb_paged_decode(const void* q, int dtype, int batch, int hq, int hk, int head_dim, const int64_t* q_strides,
+                             const void* k_cache, const void* v_cache, int cache_dtype, int num_pages, int page_size,
+                             const int64_t* cache_strides, const float* k_scale, const float* v_scale,
+                             const int64_t* scale_strides, const int32_t* page_table, int64_t table_stride,
+                             int max_pages, const int32_t* seq_lens, void* out, const int64_t* o_strides, float* lse,
+                             float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Synchronises `stream`, reads and clears the current device's paged error bits into *flags; FPB_EDEVICE if any was set. */
+FPB_API int fpb_paged_read_device_error(uint32_t* flags, void* stream);
 
 #ifdef __cplusplus
 }
