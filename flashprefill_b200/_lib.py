@@ -73,8 +73,11 @@ SIGNATURES = {
     "fpb_paged_read_device_error": (_I, [_U32P, _P]),
 }
 
+EXT_PATH = os.path.join(_HERE, "_fp_torch.so")
+
 _lock = threading.Lock()
 _lib = None
+_ext = None
 
 
 class FlashPrefillError(RuntimeError):
@@ -97,6 +100,31 @@ def load(path: str = LIB_PATH):
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def ext():
+    """The extension module that passes torch tensors to the paged-cache entry points (loaded once)."""
+    global _ext
+    if _ext is None:
+        lib = load()
+        with _lock:
+            if _ext is None:
+                if not os.path.exists(EXT_PATH):
+                    raise ImportError(
+                        f"flashprefill_b200: torch binding not built ({EXT_PATH} missing); run "
+                        "`python -m flashprefill_b200.build`")
+                import importlib.machinery
+                import importlib.util
+
+                import torch  # noqa: F401  (its libraries must be loaded first)
+                loader = importlib.machinery.ExtensionFileLoader("_fp_torch", EXT_PATH)
+                m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fp_torch", loader))
+                loader.exec_module(m)
+                addr = lambda name: ctypes.cast(getattr(lib, name), _P).value
+                m.bind(addr("fpb_kv_cache_write"), addr("fpb_kv_cache_read"), addr("fpb_paged_decode"),
+                       addr("fpb_paged_decode_workspace_bytes"), addr("fpb_last_error"), FlashPrefillError)
+                _ext = m
+    return _ext
 
 
 def i64arr(vals):

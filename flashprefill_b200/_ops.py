@@ -321,188 +321,42 @@ def attention_varlen(q, k, v, o, cu_seqlens, max_seq_len, workspace: torch.Tenso
 
 
 # --------------------------------------------------------------------------- paged cache
-def _cuda_tensor(t, name, ndim, device):
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dim() != ndim:
-        raise ValueError(f"{name} must have {ndim} dimensions, got shape {tuple(t.shape)}")
-    if t.device.type != "cuda":
-        raise ValueError(f"{name} must be a CUDA tensor (flashprefill_b200 has no CPU path), got {t.device}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-
-
-def _written(t, name):
-    """A tensor that a kernel writes must not have two indices for one element through a stride of 0."""
-    for n, s in zip(t.shape, t.stride()):
-        if s == 0 and n > 1:
-            raise ValueError(f"{name} is written to and must not be an expanded tensor (strides {tuple(t.stride())})")
-
-
-def _cache_args(k_cache, v_cache, k_scale, v_scale, dtype, device, heads, written):
-    """Checks the cache tensors; returns (cache dtype code, pages, page size, kv heads, cache strides, scale strides)."""
-    _cuda_tensor(k_cache, "k_cache", 4, device)
-    _cuda_tensor(v_cache, "v_cache", 4, device)
-    shape, strides = k_cache.shape, k_cache.stride()
-    if v_cache.shape != shape or v_cache.stride() != strides or v_cache.dtype != k_cache.dtype:
-        raise ValueError("k_cache and v_cache must share shape, strides and dtype")
-    if heads is not None and shape[2] != heads:
-        raise ValueError(f"the cache has {shape[2]} KV heads, expected {heads}")
-    if shape[3] != 128 or strides[3] != 1:
-        raise ValueError(f"the cache's last dimension must be 128 contiguous elements, got shape {tuple(shape)}, strides {strides}")
-    if written:
-        _written(k_cache, "k_cache")
-    if k_cache.dtype is torch.float8_e4m3fn:
-        if k_scale is None or v_scale is None:
-            raise ValueError("an e4m3 cache needs k_scale and v_scale")
-        _cuda_tensor(k_scale, "k_scale", 3, device)
-        _cuda_tensor(v_scale, "v_scale", 3, device)
-        if k_scale.shape != shape[:3] or v_scale.shape != shape[:3]:
-            raise ValueError(f"k_scale and v_scale must have shape {tuple(shape[:3])}")
-        if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
-            raise TypeError("k_scale and v_scale must be float32")
-        if k_scale.stride() != v_scale.stride():
-            raise ValueError("k_scale and v_scale must share strides")
-        if written:
-            _written(k_scale, "k_scale")
-        return _lib.FPB_E4M3, shape[0], shape[1], shape[2], _lib.i64arr(strides[:3]), _lib.i64arr(k_scale.stride())
-    if k_cache.dtype is not dtype:
-        raise TypeError(f"the cache must be {dtype} or torch.float8_e4m3fn, got {k_cache.dtype}")
-    if k_scale is not None or v_scale is not None:
-        raise ValueError("a 16-bit cache takes no scales")
-    return _DTYPES[dtype], shape[0], shape[1], shape[2], _lib.i64arr(strides[:3]), None
-
-
-def _table_args(page_table, seq_lens, batch, device):
-    _cuda_tensor(page_table, "page_table", 2, device)
-    _cuda_tensor(seq_lens, "seq_lens", 1, device)
-    if page_table.dtype is not torch.int32 or seq_lens.dtype is not torch.int32:
-        raise TypeError("page_table and seq_lens must be int32")
-    if page_table.shape[0] != batch or seq_lens.shape[0] != batch:
-        raise ValueError(f"page_table {tuple(page_table.shape)} and seq_lens {tuple(seq_lens.shape)} must have {batch} rows")
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1 or batch > 1 and seq_lens.stride(0) != 1:
-        raise ValueError("the last dimension of page_table and of seq_lens must be contiguous")
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _finish_paged(stream) -> None:
-    if _CHECK and not torch.cuda.is_current_stream_capturing():
-        _check_paged(stream)
-
-
-def _check_paged(stream) -> None:
+def check_paged_error(device=None) -> None:
+    """Synchronise the current stream and raise if a paged-cache call on ``device`` (default: the current one) met a slot,
+    page or length outside its tensors since the last check."""
     flags = ctypes.c_uint32(0)
-    rc = _lib.load().fpb_paged_read_device_error(ctypes.byref(flags), stream)
+    with torch.cuda.device(device):
+        rc = _lib.load().fpb_paged_read_device_error(ctypes.byref(flags), torch.cuda.current_stream().cuda_stream)
     if rc == _lib.FPB_EDEVICE:
         what = [m for b, m in _lib.DEV_ERROR_BITS.items() if flags.value & b]
         raise _lib.FlashPrefillError("flashprefill_b200 device error: " + "; ".join(what))
     _lib.check(rc)
 
 
-def check_paged_error(device=None) -> None:
-    """Synchronise the current stream and raise if a paged-cache call on ``device`` (default: the current one) met a slot,
-    page or length outside its tensors since the last check."""
-    with torch.cuda.device(device):
-        _check_paged(torch.cuda.current_stream().cuda_stream)
+def _finish_paged(device) -> None:
+    if _CHECK and not torch.cuda.is_current_stream_capturing():
+        check_paged_error(device)
 
 
-def kv_cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> None:
-    device = k.device if isinstance(k, torch.Tensor) else None
-    k = _prep_input(k, "k", 3, device)
-    v = _prep_input(v, "v", 3, device)
-    T, Hk, D = k.shape
-    if v.shape != k.shape:
-        raise ValueError(f"v shape {tuple(v.shape)} must equal k shape {tuple(k.shape)}")
-    if v.dtype != k.dtype:
-        raise TypeError("k and v must share one dtype")
-    code = _dtype_code(k)
-    ccode, pages, page_size, _, cs, ss = _cache_args(k_cache, v_cache, k_scale, v_scale, k.dtype, device, Hk, True)
-    _cuda_tensor(slots, "slots", 1, device)
-    if slots.dtype is not torch.int64 and slots.dtype is not torch.int32:
-        raise TypeError(f"slots must be int64 or int32, got {slots.dtype}")
-    if slots.shape[0] != T:
-        raise ValueError(f"slots must have one entry for each of the {T} rows, got {slots.shape[0]}")
-    slots = slots.contiguous()
+# The entry points' checks and launches are in csrc/fp_torch.cpp.
+def kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale) -> None:
+    (_lib._ext or _lib.ext()).kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
     if _CHECK and not torch.cuda.is_current_stream_capturing():
         used = slots[slots >= 0]
         if used.unique().numel() != used.numel():
             raise ValueError("two rows name one slot")
-    stream = torch.cuda.current_stream(device).cuda_stream
-    with torch.cuda.device(device):
-        rc = _lib.load().fpb_kv_cache_write(_ptr(k), _ptr(v), code, T, Hk, D, _strides(k, 2), _strides(v, 2), _ptr(k_cache),
-                                            _ptr(v_cache), ccode, pages, page_size, cs, _ptr(k_scale), _ptr(v_scale), ss,
-                                            _ptr(slots), slots.element_size(), stream)
-        _lib.check(rc)
-        _finish_paged(stream)
+        check_paged_error(k.device)
 
 
-def kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale=None, v_scale=None) -> None:
-    device = k_cache.device if isinstance(k_cache, torch.Tensor) else None
-    for t, name in ((k, "k"), (v, "v")):
-        _cuda_tensor(t, name, 4, device)
-        _written(t, name)
-        if not _tma_ok(t):
-            raise ValueError(f"{name} must have a contiguous last dimension and 16-byte aligned rows")
-    if v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError("k and v must share shape and dtype")
-    B, S, Hk, D = k.shape
-    code = _dtype_code(k)
-    ccode, pages, page_size, _, cs, ss = _cache_args(k_cache, v_cache, k_scale, v_scale, k.dtype, device, Hk, False)
-    _table_args(page_table, seq_lens, B, device)
-    if B == 0 or S == 0 or page_table.shape[1] == 0:
-        return
-    stream = torch.cuda.current_stream(device).cuda_stream
-    with torch.cuda.device(device):
-        rc = _lib.load().fpb_kv_cache_read(_ptr(k_cache), _ptr(v_cache), ccode, pages, page_size, Hk, D, cs, _ptr(k_scale),
-                                           _ptr(v_scale), ss, _ptr(page_table), page_table.stride(0), page_table.shape[1],
-                                           _ptr(seq_lens), B, _ptr(k), _ptr(v), code, S, _strides(k, 3), _strides(v, 3),
-                                           stream)
-        _lib.check(rc)
-        _finish_paged(stream)
+def kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale) -> None:
+    (_lib._ext or _lib.ext()).kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale)
+    _finish_paged(k.device)
 
 
-def paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse=None, k_scale=None, v_scale=None, sm_scale=None,
-                 workspace=None) -> None:
-    device = q.device if isinstance(q, torch.Tensor) else None
-    q = _prep_input(q, "q", 3, device)
-    B, Hq, D = q.shape
-    code = _dtype_code(q)
-    _cuda_tensor(out, "out", 3, device)
-    if out.shape != q.shape or out.dtype is not q.dtype:
-        raise ValueError("out must be a tensor with q's shape, dtype and device")
-    if out.stride(2) != 1:
-        raise ValueError("out's last dimension must be contiguous")
-    _written(out, "out")
-    ccode, pages, page_size, Hk, cs, ss = _cache_args(k_cache, v_cache, k_scale, v_scale, q.dtype, device, None, False)
-    if Hk == 0 or Hq % Hk:
-        raise ValueError(f"num_q_heads ({Hq}) must be a multiple of num_kv_heads ({Hk})")
-    _table_args(page_table, seq_lens, B, device)
-    if lse is not None:
-        _cuda_tensor(lse, "lse", 2, device)
-        if lse.shape != q.shape[:2] or lse.dtype is not torch.float32 or not lse.is_contiguous():
-            raise ValueError(f"lse must be a contiguous float32 tensor of shape {(B, Hq)}")
-    if B == 0 or Hq == 0:
-        return
-    lib = _lib.load()
-    max_pages = page_table.shape[1]
-    stream = torch.cuda.current_stream(device).cuda_stream
-    with torch.cuda.device(device):
-        if workspace is None:
-            n = lib.fpb_paged_decode_workspace_bytes(B, Hq, Hk, ccode, max_pages, page_size)
-            if n:
-                workspace = torch.empty(n, dtype=torch.uint8, device=device)
-        else:
-            _cuda_tensor(workspace, "workspace", 1, device)
-        rc = lib.fpb_paged_decode(_ptr(q), code, B, Hq, Hk, D, _strides(q, 2), _ptr(k_cache), _ptr(v_cache), ccode, pages,
-                                  page_size, cs, _ptr(k_scale), _ptr(v_scale), ss, _ptr(page_table), page_table.stride(0),
-                                  max_pages, _ptr(seq_lens), _ptr(out), _strides(out, 2), _ptr(lse),
-                                  1.0 / 128 ** 0.5 if sm_scale is None else float(sm_scale), _ptr(workspace),
-                                  0 if workspace is None else workspace.numel() * workspace.element_size(), stream)
-        _lib.check(rc)
-        _finish_paged(stream)
+def paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale, workspace) -> None:
+    (_lib._ext or _lib.ext()).paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale,
+                                           workspace)
+    _finish_paged(q.device)
 
 
 def paged_decode_workspace_bytes(batch, q_heads, kv_heads, cache_dtype, max_pages, page_size) -> int:

@@ -3,7 +3,8 @@
     python -m flashprefill_b200.build [--verbose-ptxas]
 
 The library is one unity translation unit (csrc/fp_api.cu includes the kernels) linked
-against the static CUDA runtime, so it only needs the NVIDIA driver at run time.
+against the static CUDA runtime, so it only needs the NVIDIA driver at run time.  Beside it
+_fp_torch.so (csrc/fp_torch.cpp, g++) passes torch tensors to the paged-cache entry points.
 """
 from __future__ import annotations
 
@@ -16,6 +17,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libflashprefill_b200.so")
 SOURCES = ["fp_api.cu"]
+EXT = os.path.join(HERE, "_fp_torch.so")
+EXT_SOURCE = "fp_torch.cpp"
+HEADER = os.path.join(os.path.dirname(HERE), "include", "flashprefill_b200.h")
 
 
 def nvcc_path() -> str:
@@ -27,7 +31,7 @@ def nvcc_path() -> str:
 
 def _deps():
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))]
-    deps.append(os.path.join(os.path.dirname(HERE), "include", "flashprefill_b200.h"))
+    deps.append(HEADER)
     return deps
 
 
@@ -38,7 +42,32 @@ def needs_build() -> bool:
     return any(os.path.getmtime(d) > t for d in _deps())
 
 
+def build_ext(force: bool = False) -> str:
+    """_fp_torch.so: plain g++ against torch's headers (its C++ interface has no device code)."""
+    src = os.path.join(CSRC, EXT_SOURCE)
+    if not force and os.path.exists(EXT) and all(os.path.getmtime(EXT) > os.path.getmtime(d) for d in (src, HEADER)):
+        return EXT
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    cuda = os.path.dirname(os.path.dirname(nvcc_path()))
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", EXT + ".tmp", src]
+    for d in cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]:
+        cmd += ["-isystem", d]
+    for d in cpp_extension.library_paths():
+        cmd += ["-L" + d]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+    os.replace(EXT + ".tmp", EXT)
+    return EXT
+
+
 def build(force: bool = False, ptxas_verbose: bool = False) -> str:
+    build_ext(force)
     if not force and not needs_build():
         return LIB
     cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
