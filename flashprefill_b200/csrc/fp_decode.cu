@@ -4,33 +4,38 @@
 //   s_j = sm_scale * q . k_j,   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   lse = m + log sum_j exp(s_j - m)
 //
 // for every sequence b and query head, j over the sequence's seq_lens[b] cached tokens; the G = hq / hk query heads of a
-// KV head share its rows.  Each cached byte is read once and meets 2 G flops (2-byte cache), so the operator is bound by
-// HBM; the arithmetic only has to stay out of the way.
+// KV head share its rows.  Each cached byte is read once and meets G flops (2-byte cache) or 2 G (e4m3), so the operator is
+// bound by HBM; the arithmetic only has to stay out of the way.
 //
-// Work.  An item is (sequence, KV head, group of query heads: all G up to 8 NT, equal groups above that).  All items' tokens, cut into units of
-// kWarps * TT tokens, form one line, and each of a fixed number of CTAs takes an equal stretch of it, so ragged batches
-// and single long sequences load the GPU alike, whatever the lengths (they are read on the device: no host copy, and a
-// captured graph serves any lengths).  A stretch that covers a whole item writes its output; an item cut by a CTA border
-// leaves unnormalised sums and their maxima in the workspace, which a second kernel (programmatic dependent launch)
-// joins in the order of the tokens: no atomics, the same bits on every run.  The second kernel is not launched where
-// no item can have two units.
+// An item is (sequence, KV head, group of query heads: all G up to 16, equal groups of at most 16 above that), its tokens are cut
+// into units of kDecWarps * TT.  Lengths are read on the device (no host copy; a captured graph serves any lengths).
+//
+// Long sequences (paged_decode_kernel).  All items' units form one line, and each of a fixed number of CTAs takes an equal stretch
+// of it, so ragged batches and single long sequences load the GPU alike.  A stretch that covers a whole item writes its
+// output; an item cut by a CTA border leaves unnormalised sums and their maxima in the workspace, which a second kernel
+// (programmatic dependent launch) joins in the order of the tokens.
+// Short sequences (paged_decode_short_kernel): one cluster of 1 to 8 CTAs for each item, units dealt out in turn, joined
+// through distributed shared memory.  No prefix sums, no workspace, no second kernel.
+// Both join in an order that the lengths alone decide, with no atomics: the same call gives the same bits.
 //
 // A warp works alone on its own tiles of TT tokens (16 of a 16-bit cache, 32 of e4m3: 4 KB of K and of V each way) through
-// a ring of kStages tiles filled by 16-byte cp.async, so loads are in flight all the time without block-wide barriers;
-// warps meet once an item.  Rows behind the end, or on a page that is not in the cache, are filled with zeros and their
-// scores set to -inf: stale values there never reach the sums.
+// a ring of kDecStages tiles filled by 16-byte cp.async, so loads are in flight all the time without block-wide barriers;
+// warps meet once an item.  Where page_size is a multiple of 16, 16 tokens share a page and one table entry, fetched a tile
+// ahead, gives their addresses; other page sizes look each row up.  Rows behind the end, or on a page that is not in the
+// cache, are filled with zeros and their scores set to -inf: stale values there never reach the sums.
 //
 // Tensor cores.  S^T = K Q^T with the tokens as the 16 rows and 8 heads as the columns of mma.m16n8k16; out^T = V^T P^T
 // with the channels as rows.  The small side of both products is the 8-wide one, so G <= 8 heads cost one pass where
 // tcgen05's least tile would be mostly padding, and the operands need no staging beyond the ring.
-//   * Scores, maxima, sums and outputs stay in fp32 registers; running maximum, rescaled only when it moves.
+//   * Scores, maxima, sums and outputs stay in fp32 registers.  The running maximum is reduced over the warp, and sums are
+//     rescaled, only in tiles where some score exceeds it.
 //   * bf16 V: P is split into two bf16 parts (the value and its remainder) and multiplied twice: one bf16 P would leave
 //     errors as large as the output's own rounding.
 //   * fp16 V: P is scaled by 2^15 (as the row sum is, so it cancels), which keeps weights down to 2^-29 of the largest in
 //     fp16's normal range.
 //   * e4m3: codes widen to fp16 exactly; q is scaled by a power of two to fit fp16; the token's K scale multiplies its
-//     score and its V scale its weight, relative to the largest V scale so far (a power-free running reference like the
-//     maximum), so weights stay at most 2^15.
+//     score and its V scale its weight, relative to the largest V scale so far (a running reference like the maximum), so
+//     weights stay at most 2^15.
 #include <type_traits>
 
 #include "fp_common.cuh"
@@ -38,13 +43,15 @@
 namespace fpb {
 
 constexpr int kDecWarps = 4;
-constexpr int kDecStages = 3;
+constexpr int kDecStages = 2;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kDecTileBytes = 4096;  // one warp's tile of K or of V
 constexpr int kDecRingBytes = kDecStages * 2 * kDecTileBytes;
 constexpr int kDecSmemBytes = kDecWarps * kDecRingBytes;
-constexpr int kDecCtasPerSm = 2;
+constexpr int dec_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }  // registers: 168 or 255 a thread
 constexpr int kDecMaxCtas = 512;   // bound of the workspace
+constexpr int kDecMaxCluster = 8;
+static_assert(kDecThreads == kHeadDim, "one thread for each channel in the merges");
 constexpr int kJoinThreads = 512;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -57,6 +64,8 @@ struct DecodeArgs {
   const int* page_table;
   int64_t table_stride;
   const int* seq_lens;
+  unsigned page_mul;                 // token / page_size = token * page_mul >> page_shift
+  int page_shift, page16;            // page16: page_size is a multiple of 16
   int max_pages, batch, hq, hk;
   int G, ngroups, nh;                // query heads of a KV head, groups of them, heads of a group (the last may have fewer)
   float c;                           // sm_scale * log2(e)
@@ -97,6 +106,18 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Reads the float at this CTA's shared address `addr` in CTA `rank` of the cluster.
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
 // Tokens of sequence b; a length outside [0, room] is reported and counts as 0.
@@ -109,6 +130,10 @@ __device__ __forceinline__ int seq_len_of(const DecodeArgs& A, int b) {
   return len;
 }
 
+__device__ __forceinline__ int page_of(const DecodeArgs& A, int tok) {
+  return (int)(((uint64_t)(unsigned)tok * A.page_mul) >> A.page_shift);
+}
+
 // T: type of q and out; kE4m3: codes in the cache (else T); NT: groups of 8 heads of an item.
 template <typename T, bool kE4m3, int NT>
 struct DecodeWarp {
@@ -117,6 +142,7 @@ struct DecodeWarp {
   static constexpr int MTILES = TT / 16;
   static constexpr int kRowBytes = kDecTileBytes / TT;
   static constexpr int kChunks = kRowBytes / 16;  // 16-byte pieces of a row
+  static constexpr uint32_t kFull = TT == 32 ? 0xFFFFFFFFu : 0xFFFFu;
   static constexpr bool kSplitP = DT<MT>::is_bf16;
   static constexpr float kShift = kSplitP ? 0.f : 15.f;  // log2 of the factor of P and l
 
@@ -126,7 +152,7 @@ struct DecodeWarp {
   float qc[NT][2];            // factor of this thread's two columns (heads 2t, 2t + 1)
   float o[NT][8][4];          // out^T: 16 channels x 8 heads a tile
   float m[NT][2], l[NT][2];   // running maximum and this thread's share of the sum
-  float vref;                 // e4m3: largest V scale so far
+  float vref, vinv;           // e4m3: largest V scale so far and its reciprocal
 
   __device__ __forceinline__ void load_q(const DecodeArgs& A, const uint8_t* q, int heads) {
     const int g = lane >> 2, t = lane & 3;
@@ -184,22 +210,72 @@ struct DecodeWarp {
         for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
     }
     vref = 1.1754943508222875e-38f;
+    vinv = 1.f / vref;
   }
 
-  // Starts the copies of tokens [tok, tok + TT) below `end` into ring slot `stage`; kvalid: bit r set where row r is there;
-  // ks, vs: this lane's token's scales.
+  // Table entries of the tile at `tok` (one for each 16 tokens).  Entries behind the sequence may be read, never used.
+  __device__ __forceinline__ void load_pages(const DecodeArgs& A, const int* table, int tok, int (&page)[MTILES]) {
+#pragma unroll
+    for (int j = 0; j < MTILES; ++j) {
+      const int p = page_of(A, tok + 16 * j);
+      page[j] = p < A.max_pages ? __ldg(table + p) : -1;
+    }
+  }
+
+  // Starts the copies of tokens [tok, tok + TT) below `end` into ring slot `stage`.  valid: bit r set where row r is there;
+  // ks, vs: the scales of this lane's token.
   __device__ __forceinline__ void issue(const DecodeArgs& A, const int* table, int64_t head_off, int64_t scale_off, int tok,
-                                        int end, int stage, uint32_t& kvalid, float& ks, float& vs) {
-    const int r0 = lane % TT, my = tok + r0;
-    int64_t off = -1;
+                                        int end, int stage, const int (&page)[MTILES], uint32_t& valid, float& ks, float& vs) {
+    constexpr int kRowsPer = 32 / kChunks;  // rows of one copy instruction of the warp
+    const uint32_t kd = ring + stage * 2 * kDecTileBytes, vd = kd + kDecTileBytes;
+    const int ch = lane % kChunks, r0 = lane / kChunks;
     ks = vs = 0.f;
-    if (my < end) {
-      const int p = my / A.C.page_size, at = my - p * A.C.page_size;
-      const int page = __ldg(table + p);
-      if (page >= 0 && page < A.C.num_pages) {
-        off = (int64_t)page * A.C.s_page + (int64_t)at * A.C.s_tok;
+    if (A.page16) {
+      valid = 0;
+#pragma unroll
+      for (int j = 0; j < MTILES; ++j) {
+        const int t0 = tok + 16 * j;
+        int rows = max(0, min(16, end - t0));
+        int64_t pg = page[j];
+        if (rows > 0 && (unsigned)page[j] >= (unsigned)A.C.num_pages) {
+          raise_error(&g_paged_err, kErrBadPage);
+          rows = 0;
+        }
+        if (rows == 0) pg = 0;
+        const int at = rows == 0 ? 0 : t0 - page_of(A, t0) * A.C.page_size;
+        valid |= ((1u << rows) - 1u) << (16 * j);
+        const int64_t off = pg * A.C.s_page + (int64_t)(at + r0) * A.C.s_tok + head_off + ch * 16;
+        const uint8_t* kp = A.C.k + off;
+        const uint8_t* vp = A.C.v + off;
+        const int64_t step = kRowsPer * A.C.s_tok;
+#pragma unroll
+        for (int i = 0; i < 16 / kRowsPer; ++i) {
+          const int r = i * kRowsPer + r0, row = 16 * j + r;
+          const uint32_t d = row * kRowBytes + ((ch ^ (row & 7)) << 4);
+          const int bytes = r < rows ? 16 : 0;  // rows behind the end lie on the same page
+          cp_async16(kd + d, kp, bytes);
+          cp_async16(vd + d, vp, bytes);
+          kp += step;
+          vp += step;
+        }
         if constexpr (kE4m3) {
-          const int64_t so = (int64_t)page * A.C.ss_page + (int64_t)at * A.C.ss_tok + scale_off;
+          if (lane / 16 == j && lane % 16 < rows) {
+            const int64_t so = pg * A.C.ss_page + (int64_t)(at + lane % 16) * A.C.ss_tok + scale_off;
+            ks = __ldg(A.C.k_scale + so);
+            vs = __ldg(A.C.v_scale + so);
+          }
+        }
+      }
+      return;
+    }
+    const int my = tok + lane % TT;
+    int64_t off = -1;
+    if (my < end) {
+      const int p = page_of(A, my), at = my - p * A.C.page_size, pg = __ldg(table + p);
+      if ((unsigned)pg < (unsigned)A.C.num_pages) {
+        off = (int64_t)pg * A.C.s_page + (int64_t)at * A.C.s_tok;
+        if constexpr (kE4m3) {
+          const int64_t so = (int64_t)pg * A.C.ss_page + (int64_t)at * A.C.ss_tok + scale_off;
           ks = __ldg(A.C.k_scale + so);
           vs = __ldg(A.C.v_scale + so);
         }
@@ -207,13 +283,11 @@ struct DecodeWarp {
         raise_error(&g_paged_err, kErrBadPage);
       }
     }
-    kvalid = __ballot_sync(0xffffffffu, off >= 0);
-    const uint32_t kd = ring + stage * 2 * kDecTileBytes, vd = kd + kDecTileBytes;
-    const int ch = lane % kChunks;
-    constexpr int kRowsPer = 32 / kChunks;
-#pragma unroll
+    valid = __ballot_sync(0xffffffffu, off >= 0);
+    if constexpr (TT == 16) valid &= 0xFFFFu;
+#pragma unroll 1
     for (int i = 0; i < TT / kRowsPer; ++i) {
-      const int r = i * kRowsPer + lane / kChunks;
+      const int r = i * kRowsPer + r0;
       const int64_t ro = __shfl_sync(0xffffffffu, off, r);
       const uint32_t d = r * kRowBytes + ((ch ^ (r & 7)) << 4);
       const int64_t so = ro < 0 ? 0 : ro + head_off + ch * 16;
@@ -222,108 +296,136 @@ struct DecodeWarp {
     }
   }
 
-  __device__ __forceinline__ void consume(int stage, uint32_t kvalid, float ks, float vs) {
+  __device__ __forceinline__ void consume(int stage, uint32_t valid, float ks, float vs) {
     const uint32_t kd = ring + stage * 2 * kDecTileBytes, vd = kd + kDecTileBytes;
     const int g = lane >> 2;
     float s[NT][MTILES][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < MTILES; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][i][j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint32_t a[4];
-      if constexpr (!kE4m3) {
-        const int r = lane & 15, ch = 2 * k + (lane >> 4);
-        ldsm4(a, kd + r * kRowBytes + ((ch ^ (r & 7)) << 4));
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<MT>(s[n][0], a[0], a[1], a[2], a[3], qf[n][k][0], qf[n][k][1]);
-      } else {
-        ldsm4(a, kd + lane * kRowBytes + ((k ^ (lane & 7)) << 4));
-#pragma unroll
-        for (int i = 0; i < MTILES; ++i) {
-          const uint32_t a0 = e4m3x2_to_f16x2(a[2 * i]), a2 = e4m3x2_to_f16x2(a[2 * i] >> 16);
-          const uint32_t a1 = e4m3x2_to_f16x2(a[2 * i + 1]), a3 = e4m3x2_to_f16x2(a[2 * i + 1] >> 16);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<MT>(s[n][i], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
-        }
-      }
-    }
-    // row factors of this thread's tokens g, g + 8 (+ 16 i)
-    float kf[MTILES][2], vf[MTILES][2];
-    float vcorr = 1.f;
-    if constexpr (kE4m3) {
-      const float vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vs)));
-      const float vnew = vmax > vref || vmax != vmax ? vmax : vref;
-      vcorr = vref / vnew;
-      vref = vnew;
-      const float vw = vs / vnew;
-#pragma unroll
-      for (int i = 0; i < MTILES; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          kf[i][j] = __shfl_sync(0xffffffffu, ks, 16 * i + 8 * j + g);
-          vf[i][j] = __shfl_sync(0xffffffffu, vw, 16 * i + 8 * j + g);
-        }
-    }
-    bool moved = vcorr != 1.f;
-    float corr[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {  // the column (head) 2t + j
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < MTILES; ++i) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x = s[n][i][2 * h + j] * qc[n][j];
-            if constexpr (kE4m3) x *= kf[i][h];
-            x = (kvalid >> (16 * i + 8 * h + g)) & 1u ? x : -INFINITY;
-            s[n][i][2 * h + j] = x;
-            mx = fmaxf(mx, x);
-          }
-        }
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        const float mn = fmaxf(m[n][j], mx), ref = finite_or_zero(mn);
-        moved |= mn != m[n][j];
-        const float cr = ex2_approx(m[n][j] - ref);
-        m[n][j] = mn;
-        l[n][j] *= cr;
-        corr[n][j] = cr * vcorr;
-#pragma unroll
-        for (int i = 0; i < MTILES; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float p = ex2_approx(s[n][i][2 * h + j] - (ref - kShift));
-            l[n][j] += p;
-            s[n][i][2 * h + j] = kE4m3 ? p * vf[i][h] : p;
-          }
-      }
-    }
-    if (__any_sync(0xffffffffu, moved)) {
+    {
+      float s2[NT][4];  // second chain of products of a 16-token tile (32 tokens have two as it is)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int j = 0; j < 4; ++j) {
+          s2[n][j] = 0.f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o[n][i][j] *= corr[n][j & 1];
+          for (int i = 0; i < MTILES; ++i) s[n][i][j] = 0.f;
+        }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t a[4];
+        if constexpr (!kE4m3) {
+          const int r = lane & 15, ch = 2 * k + (lane >> 4);
+          ldsm4(a, kd + r * kRowBytes + ((ch ^ (r & 7)) << 4));
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            mma16816<MT>(k & 1 ? s2[n] : s[n][0], a[0], a[1], a[2], a[3], qf[n][k][0], qf[n][k][1]);
+        } else {
+          ldsm4(a, kd + lane * kRowBytes + ((k ^ (lane & 7)) << 4));
+#pragma unroll
+          for (int i = 0; i < MTILES; ++i) {
+            const uint32_t a0 = e4m3x2_to_f16x2(a[2 * i]), a2 = e4m3x2_to_f16x2(a[2 * i] >> 16);
+            const uint32_t a1 = e4m3x2_to_f16x2(a[2 * i + 1]), a3 = e4m3x2_to_f16x2(a[2 * i + 1] >> 16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<MT>(s[n][i], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+          }
+        }
+      }
+      if constexpr (!kE4m3) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[n][0][j] += s2[n][j];
+      }
     }
-    uint32_t pb[NT][MTILES][2], pl[NT][MTILES][2];
+    // scores in log2 units; the largest of this thread's rows g, g + 8 (+ 16 i) for its columns 2t + j
+    bool moved = false;
+    float mx[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float kf = 1.f;
+        if constexpr (kE4m3) kf = __shfl_sync(0xffffffffu, ks, 16 * i + 8 * h + g);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float& x = s[n][i][2 * h + j];
+            x *= qc[n][j];
+            if constexpr (kE4m3) x *= kf;
+          }
+      }
+    if (valid != kFull) {
 #pragma unroll
       for (int i = 0; i < MTILES; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x0 = s[n][i][2 * h], x1 = s[n][i][2 * h + 1];
-          const uint32_t hi = DT<MT>::pack(x0, x1);
-          pb[n][i][h] = transpose8x8(hi);
-          if constexpr (kSplitP) pl[n][i][h] = transpose8x8(DT<MT>::pack(x0 - DT<MT>::lo(hi), x1 - DT<MT>::hi(hi)));
+        for (int h = 0; h < 2; ++h)
+          if (!((valid >> (16 * i + 8 * h + g)) & 1u)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][i][2 * h] = s[n][i][2 * h + 1] = -INFINITY;
+          }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < MTILES; ++i) mx[n][j] = fmaxf(mx[n][j], fmaxf(s[n][i][j], s[n][i][2 + j]));
+        moved |= mx[n][j] > m[n][j];
+      }
+    if constexpr (kE4m3) moved |= !(vs <= vref);
+    if (__any_sync(0xffffffffu, moved)) {
+      float vcorr = 1.f;
+      if constexpr (kE4m3) {
+        const float vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vs)));
+        const float vnew = vmax <= vref ? vref : vmax;
+        vcorr = vnew == vref ? 1.f : vref / vnew;
+        vref = vnew;
+        vinv = 1.f / vnew;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float corr[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float x = mx[n][j];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+          const float mn = fmaxf(m[n][j], x), f = ex2_approx(m[n][j] - finite_or_zero(mn));
+          m[n][j] = mn;
+          l[n][j] *= f;
+          corr[j] = f * vcorr;
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][i][j] *= corr[j & 1];
+      }
+    }
+    uint32_t pb[NT][MTILES][2], pl[NT][MTILES][2];
+    const float vw = kE4m3 ? vs * vinv : 0.f;
+#pragma unroll
+    for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float vf = 1.f;
+        if constexpr (kE4m3) vf = __shfl_sync(0xffffffffu, vw, 16 * i + 8 * h + g);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float p[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            p[j] = ex2_approx(s[n][i][2 * h + j] - (finite_or_zero(m[n][j]) - kShift));
+            l[n][j] += p[j];
+            if constexpr (kE4m3) p[j] *= vf;
+          }
+          const uint32_t hi = DT<MT>::pack(p[0], p[1]);
+          pb[n][i][h] = transpose8x8(hi);
+          if constexpr (kSplitP) pl[n][i][h] = transpose8x8(DT<MT>::pack(p[0] - DT<MT>::lo(hi), p[1] - DT<MT>::hi(hi)));
+        }
+      }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {  // 16 channels
       uint32_t a[4];
@@ -351,6 +453,54 @@ struct DecodeWarp {
     }
   }
 
+  // All of this warp's tiles of an item: tokens [tok + i * step, + TT) below min(end, the sequence's length).  The first
+  // table entries and q are on their way before the length is needed.
+  __device__ __forceinline__ void run(const DecodeArgs& A, int b, int64_t head_off, int64_t scale_off, int head0, int heads,
+                                      int tok, int step, int end) {
+    const int* table = A.page_table + b * A.table_stride;
+    int page[MTILES];
+    load_pages(A, table, tok, page);
+    load_q(A, A.q + b * A.q_b + head0 * A.q_h, heads);
+    reset();
+    const int n = end > tok ? (end - tok + step - 1) / step : 0;
+    uint32_t valid[kDecStages];
+    float ks[kDecStages], vs[kDecStages];
+#pragma unroll
+    for (int i = 0; i < kDecStages - 1; ++i) {
+      if (i < n) {
+        int cur[MTILES];
+#pragma unroll
+        for (int j = 0; j < MTILES; ++j) cur[j] = page[j];
+        if (i + 1 < n) load_pages(A, table, tok + (i + 1) * step, page);
+        issue(A, table, head_off, scale_off, tok + i * step, end, i, cur, valid[i], ks[i], vs[i]);
+      }
+      cp_async_commit();
+    }
+    for (int i0 = 0; i0 < n; i0 += kDecStages) {
+#pragma unroll
+      for (int j = 0; j < kDecStages; ++j) {
+        if (i0 + j < n) {
+          cp_async_wait<kDecStages - 2>();
+          __syncwarp();
+          constexpr int kAhead = kDecStages - 1;
+          const int st = (j + kAhead) % kDecStages, nx = i0 + j + kAhead;
+          if (nx < n) {
+            int cur[MTILES];
+#pragma unroll
+            for (int x = 0; x < MTILES; ++x) cur[x] = page[x];
+            if (nx + 1 < n) load_pages(A, table, tok + (nx + 1) * step, page);
+            issue(A, table, head_off, scale_off, tok + nx * step, end, st, cur, valid[st], ks[st], vs[st]);
+          }
+          cp_async_commit();
+          consume(j, valid[j], ks[j], vs[j]);
+          __syncwarp();
+        }
+      }
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+  }
+
   // Sums and maxima into shared memory: rows of 132 floats for each head (conflict-free), {maximum, sum} beside them.
   __device__ __forceinline__ void store(float* so, float2* sml) {
     const int g = lane >> 2, t = lane & 3;
@@ -374,8 +524,31 @@ struct DecodeWarp {
   }
 };
 
+// Joins the warps' sums of head i at channel tid: {sum of weights times v, sum of weights, maximum}.
+template <int NT>
+__device__ __forceinline__ void merge_warps(const uint8_t* smem, const float2 (&s_ml)[kDecWarps][8 * NT], int i, int tid,
+                                            float& x, float& l, float& mx) {
+  mx = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kDecWarps; ++k) mx = fmaxf(mx, s_ml[k][i].x);
+  const float ref = finite_or_zero(mx);
+  l = x = 0.f;
+#pragma unroll
+  for (int k = 0; k < kDecWarps; ++k) {
+    const float f = ex2_approx(s_ml[k][i].x - ref);
+    l += f * s_ml[k][i].y;
+    x += f * reinterpret_cast<const float*>(smem + k * kDecRingBytes)[i * 132 + tid];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_head(const DecodeArgs& A, int b, int head, int tid, float x, float l, float mx) {
+  reinterpret_cast<T*>(A.out + b * A.o_b + head * A.o_h)[tid] = DT<T>::from_f(l == 0.f ? 0.f : x / l);
+  if (A.lse && tid == 0) A.lse[(int64_t)b * A.hq + head] = l == 0.f ? -INFINITY : (mx + log2f(l)) * kLn2;
+}
+
 template <typename T, bool kE4m3, int NT>
-__global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kernel(const DecodeArgs A) {
+__global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode_kernel(const DecodeArgs A) {
   using W = DecodeWarp<T, kE4m3, NT>;
   constexpr int kUnit = kDecWarps * W::TT;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -410,7 +583,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
   incl += before;
   total *= HH;
   const int64_t ctas = min((int64_t)gridDim.x, total);
-  if (A.desc && tid == 0) A.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (tid == 0) A.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
   if ((int64_t)blockIdx.x >= ctas) return;
   int64_t t = (int64_t)blockIdx.x * total / ctas;
   const int64_t t_end = ((int64_t)blockIdx.x + 1) * total / ctas;
@@ -444,61 +617,17 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
     const int u_end = (int)min((int64_t)units, u + (t_end - t));
     const int h = hh / A.ngroups, grp = hh - h * A.ngroups;
     const int head0 = h * A.G + grp * A.nh, heads = min(A.nh, A.G - grp * A.nh);
-    const int tok0 = u * kUnit, end = min(len, u_end * kUnit);
-    const int* table = A.page_table + b * A.table_stride;
-    const int64_t head_off = h * A.C.s_head, scale_off = h * A.C.ss_head;
-    const int tiles = (end - tok0 + W::TT - 1) / W::TT;           // of the stretch (<= 0: none)
-    const int n = tiles > warp ? (tiles - warp + kDecWarps - 1) / kDecWarps : 0;  // of this warp
-
-    uint32_t valid[kDecStages];
-    float ks[kDecStages], vs[kDecStages];
-#pragma unroll
-    for (int i = 0; i < kDecStages - 1; ++i) {
-      if (i < n) w.issue(A, table, head_off, scale_off, tok0 + (i * kDecWarps + warp) * W::TT, end, i, valid[i], ks[i], vs[i]);
-      cp_async_commit();
-    }
-    w.load_q(A, A.q + b * A.q_b + head0 * A.q_h, heads);
-    w.reset();
-    for (int i0 = 0; i0 < n; i0 += kDecStages) {
-#pragma unroll
-      for (int j = 0; j < kDecStages; ++j) {
-        if (i0 + j < n) {
-          cp_async_wait<kDecStages - 2>();
-          __syncwarp();
-          const int nx = i0 + j + kDecStages - 1;
-          constexpr int kBack = kDecStages - 1;
-          const int st = (j + kBack) % kDecStages;
-          if (nx < n)
-            w.issue(A, table, head_off, scale_off, tok0 + (nx * kDecWarps + warp) * W::TT, end, st, valid[st], ks[st], vs[st]);
-          cp_async_commit();
-          w.consume(j, valid[j], ks[j], vs[j]);
-          __syncwarp();
-        }
-      }
-    }
-    cp_async_wait<0>();
-    __syncwarp();
+    w.run(A, b, h * A.C.s_head, h * A.C.ss_head, head0, heads, u * kUnit + warp * W::TT, kUnit, min(len, u_end * kUnit));
     w.store(so, s_ml[warp]);
     __syncthreads();
 
     const bool whole = u == 0 && u_end == units;
     const int slot = 2 * blockIdx.x + (u == 0 ? 1 : 0);
     for (int i = 0; i < heads; ++i) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < kDecWarps; ++k) mx = fmaxf(mx, s_ml[k][i].x);
-      const float ref = finite_or_zero(mx);
-      float l = 0.f, x = 0.f;
-#pragma unroll
-      for (int k = 0; k < kDecWarps; ++k) {
-        const float f = ex2_approx(s_ml[k][i].x - ref);
-        l += f * s_ml[k][i].y;
-        x += f * reinterpret_cast<const float*>(smem + k * kDecRingBytes)[i * 132 + tid];
-      }
+      float x, l, mx;
+      merge_warps<NT>(smem, s_ml, i, tid, x, l, mx);
       if (whole) {
-        const int head = head0 + i;
-        reinterpret_cast<T*>(A.out + b * A.o_b + head * A.o_h)[tid] = DT<T>::from_f(l == 0.f ? 0.f : x / l);
-        if (A.lse && tid == 0) A.lse[(int64_t)b * A.hq + head] = l == 0.f ? -INFINITY : (mx + log2f(l)) * kLn2;
+        write_head<T>(A, b, head0 + i, tid, x, l, mx);
       } else {
         A.part[((int64_t)slot * A.nh + i) * kHeadDim + tid] = x;
         if (tid == 0) A.ml[(int64_t)slot * A.nh + i] = make_float2(mx, l);
@@ -523,36 +652,102 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
   }
 }
 
+// One item for each cluster of `cluster` CTAs (a power of two up to 8); CTA r takes the units r, r + cluster, ...
+template <typename T, bool kE4m3, int NT>
+__global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode_short_kernel(const DecodeArgs A, int cluster) {
+  using W = DecodeWarp<T, kE4m3, NT>;
+  constexpr int kUnit = kDecWarps * W::TT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 s_ml[kDecWarps][8 * NT];
+  __shared__ float s_x[8 * NT][kHeadDim];  // this CTA's sums, read by the others of the cluster
+  __shared__ float2 s_cta[8 * NT];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int item = blockIdx.x / cluster, rank = blockIdx.x - item * cluster;
+  const int HH = A.hk * A.ngroups, b = item / HH, hh = item - b * HH;
+  const int h = hh / A.ngroups, grp = hh - h * A.ngroups;
+  const int head0 = h * A.G + grp * A.nh, heads = min(A.nh, A.G - grp * A.nh);
+  W w;
+  w.lane = lane;
+  w.ring = smem_u32(smem) + warp * kDecRingBytes;
+  w.run(A, b, h * A.C.s_head, h * A.C.ss_head, head0, heads, rank * kUnit + warp * W::TT, cluster * kUnit, seq_len_of(A, b));
+  w.store(reinterpret_cast<float*>(smem + warp * kDecRingBytes), s_ml[warp]);
+  __syncthreads();
+  for (int i = 0; i < heads; ++i) {
+    float x, l, mx;
+    merge_warps<NT>(smem, s_ml, i, tid, x, l, mx);
+    if (cluster == 1) {
+      write_head<T>(A, b, head0 + i, tid, x, l, mx);
+    } else {
+      s_x[i][tid] = x;
+      if (tid == 0) s_cta[i] = make_float2(mx, l);
+    }
+  }
+  if (cluster == 1) return;
+  cluster_sync();
+  for (int i = rank; i < heads; i += cluster) {
+    const uint32_t ax = smem_u32(&s_x[i][tid]), am = smem_u32(&s_cta[i]);
+    float2 ml[kDecMaxCluster];
+    float xs[kDecMaxCluster], mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kDecMaxCluster; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      xs[k] = 0.f;
+      if (k < cluster) {
+        ml[k] = make_float2(ld_cluster(am, k), ld_cluster(am + 4, k));
+        xs[k] = ld_cluster(ax, k);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kDecMaxCluster; ++k) mx = fmaxf(mx, ml[k].x);
+    const float ref = finite_or_zero(mx);
+    float l = 0.f, x = 0.f;
+#pragma unroll
+    for (int k = 0; k < kDecMaxCluster; ++k) {
+      const float f = ex2_approx(ml[k].x - ref);
+      l += f * ml[k].y;
+      x += f * xs[k];
+    }
+    write_head<T>(A, b, head0 + i, tid, x, l, mx);
+  }
+  cluster_sync();  // no CTA leaves while others read its sums
+}
+
 // Joins the partial sums of the item that CTA blockIdx.x of the first kernel began and did not end.  A warp takes one head
 // and every parts-th partial (all maxima first, then the weighted sums, four channels a lane); the parts meet in shared
-// memory.
+// memory.  What the first loads need does not depend on the description, so they travel together.
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_decode_join_kernel(const DecodeArgs A) {
-  __shared__ float s_x[kJoinThreads / 32][kHeadDim];
-  __shared__ float s_l[kJoinThreads / 32];
+  constexpr int kWarps = kJoinThreads / 32;
+  __shared__ float s_x[kWarps][kHeadDim];
+  __shared__ float s_l[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int parts = kWarps / A.nh;  // nh <= 16
+  const int i = warp % A.nh, part = warp / A.nh;
+  const int room = gridDim.x - blockIdx.x;
+  auto slot = [&](int k) { return (int64_t)(2 * (blockIdx.x + k) + (k == 0 ? 1 : 0)) * A.nh + i; };
+  auto sums = [&](int k) { return reinterpret_cast<const float4*>(A.part + slot(k) * kHeadDim)[lane]; };
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 d = A.desc[blockIdx.x];
+  const float2 early = lane < room ? A.ml[slot(lane)] : make_float2(-INFINITY, 0.f);
+  const float4 first = part < min(parts, room) ? sums(part) : make_float4(0.f, 0.f, 0.f, 0.f);
   const int n = d.z;
   if (n == 0) return;
   const int b = d.x, h = d.y / A.ngroups, grp = d.y - h * A.ngroups;
   const int head0 = h * A.G + grp * A.nh, heads = min(A.nh, A.G - grp * A.nh);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int kWarps = kJoinThreads / 32;
-  const int parts = kWarps / heads;  // heads <= 16
-  const int i = warp % heads, part = warp / heads;
-  auto slot = [&](int k) { return (int64_t)(2 * (blockIdx.x + k) + (k == 0 ? 1 : 0)) * A.nh + i; };
-  float mx = -INFINITY;
-  for (int k = lane; k < n; k += 32) mx = fmaxf(mx, A.ml[slot(k)].x);
+  const bool mine = part < parts && i < heads;
+  float mx = lane < n ? early.x : -INFINITY;
+  for (int k = lane + 32; k < n; k += 32) mx = fmaxf(mx, A.ml[slot(k)].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const float ref = finite_or_zero(mx);
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
-  if (part < parts) {
+  if (mine) {
 #pragma unroll 8
     for (int k = part; k < n; k += parts) {
-      const float2 ml = A.ml[slot(k)];
-      const float4 p = reinterpret_cast<const float4*>(A.part + slot(k) * kHeadDim)[lane];
+      const float em = __shfl_sync(0xffffffffu, early.x, k & 31), el = __shfl_sync(0xffffffffu, early.y, k & 31);
+      const float2 ml = k < 32 ? make_float2(em, el) : A.ml[slot(k)];
+      const float4 p = k == part ? first : sums(k);
       const float f = ex2_approx(ml.x - ref);
       l += f * ml.y;
       x.x += f * p.x;
@@ -564,22 +759,23 @@ __global__ void __launch_bounds__(kJoinThreads) paged_decode_join_kernel(const D
     if (lane == 0) s_l[warp] = l;
   }
   __syncthreads();
-  if (part != 0) return;
+  if (!mine || part != 0) return;
   for (int k = 1; k < parts; ++k) {
-    const float4 p = reinterpret_cast<const float4*>(s_x[warp + k * heads])[lane];
-    l += s_l[warp + k * heads];
+    const float4 p = reinterpret_cast<const float4*>(s_x[warp + k * A.nh])[lane];
+    l += s_l[warp + k * A.nh];
     x.x += p.x;
     x.y += p.y;
     x.z += p.z;
     x.w += p.w;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* out = reinterpret_cast<T*>(A.out + b * A.o_b + (head0 + i) * A.o_h) + 4 * lane;
+  const float inv = 1.f / l;
   if (l == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
-  out[0] = DT<T>::from_f(x.x * inv);
-  out[1] = DT<T>::from_f(x.y * inv);
-  out[2] = DT<T>::from_f(x.z * inv);
-  out[3] = DT<T>::from_f(x.w * inv);
+  const float f = l == 0.f ? 0.f : inv;
+  T* out = reinterpret_cast<T*>(A.out + b * A.o_b + (head0 + i) * A.o_h) + 4 * lane;
+  out[0] = DT<T>::from_f(x.x * f);
+  out[1] = DT<T>::from_f(x.y * f);
+  out[2] = DT<T>::from_f(x.z * f);
+  out[3] = DT<T>::from_f(x.w * f);
   if (A.lse && lane == 0) A.lse[(int64_t)b * A.hq + head0 + i] = l == 0.f ? -INFINITY : (mx + log2f(l)) * kLn2;
 }
 

@@ -67,20 +67,25 @@ void head_groups(int G, int* ngroups, int* nh) {
   *ngroups = (G + *nh - 1) / *nh;
 }
 
-// Units that an item can have, and the CTAs that can have work.
+// How a call runs.  Short sequences: clusters of the least power of two of CTAs that fills the GPU's places (at most 8, and
+// no more than an item can have units), if that leaves at most kShortUnits units to a CTA; else equal stretches of all units.
+constexpr int kShortUnits = 16;
+constexpr int kDecPlaces = 148 * 3;
 struct DecodeShape {
-  int G, ngroups, nh, unit, max_ctas;
-  bool split;
+  int G, ngroups, nh, max_ctas, cluster;  // cluster: 0 for stretches
+  int64_t items;
 };
 DecodeShape decode_shape(int batch, int hq, int hk, int cache_dtype, int max_pages, int page_size) {
   DecodeShape s{};
   s.G = hq / hk;
   head_groups(s.G, &s.ngroups, &s.nh);
-  s.unit = kDecWarps * (cache_dtype == FPB_E4M3 ? 32 : 16);
-  const int64_t units = ((int64_t)max_pages * page_size + s.unit - 1) / s.unit;
-  s.split = units > 1;
-  const int64_t items = (int64_t)batch * hk * s.ngroups;
-  s.max_ctas = (int)std::min<int64_t>(kDecMaxCtas, units >= kDecMaxCtas ? kDecMaxCtas : items * units);
+  const int unit = kDecWarps * (cache_dtype == FPB_E4M3 ? 32 : 16);
+  const int64_t units = ((int64_t)max_pages * page_size + unit - 1) / unit;
+  s.items = (int64_t)batch * hk * s.ngroups;
+  int cluster = 1;
+  while (cluster < kDecMaxCluster && 2 * cluster <= units && s.items * cluster < kDecPlaces) cluster *= 2;
+  s.cluster = (units + cluster - 1) / cluster <= kShortUnits && s.items * cluster < (int64_t(1) << 31) ? cluster : 0;
+  s.max_ctas = (int)std::min<int64_t>(kDecMaxCtas, units >= kDecMaxCtas ? kDecMaxCtas : s.items * units);
   return s;
 }
 int64_t decode_ws_part(const DecodeShape& s) { return align256(16 * (int64_t)s.max_ctas); }
@@ -88,24 +93,38 @@ int64_t decode_ws_ml(const DecodeShape& s) {
   return decode_ws_part(s) + align256(2 * (int64_t)s.max_ctas * s.nh * kHeadDim * 4);
 }
 int64_t decode_ws_total(const DecodeShape& s) {
-  return s.split ? decode_ws_ml(s) + align256(2 * (int64_t)s.max_ctas * s.nh * 8) : 0;
+  return s.cluster ? 0 : decode_ws_ml(s) + align256(2 * (int64_t)s.max_ctas * s.nh * 8);
 }
 
 template <typename T, bool kE4m3, int NT>
-int launch_decode(const DecodeArgs& A, int ctas, bool split, cudaStream_t stream) {
+int launch_decode(const DecodeArgs& A, const DecodeShape& s, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.blockDim = dim3(kDecThreads);
+  cfg.dynamicSmemBytes = kDecSmemBytes;
+  if (s.cluster) {
+    auto kernel = paged_decode_short_kernel<T, kE4m3, NT>;
+    FPB_TRY(set_smem(kernel, kDecSmemBytes));
+    cfg.gridDim = dim3((unsigned)(s.items * s.cluster));
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = s.cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.numAttrs = s.cluster > 1;
+    FPB_CUDA(cudaLaunchKernelEx(&cfg, kernel, A, s.cluster));
+    return FPB_OK;
+  }
   auto kernel = paged_decode_kernel<T, kE4m3, NT>;
   FPB_TRY(set_smem(kernel, kDecSmemBytes));
-  kernel<<<ctas, kDecThreads, kDecSmemBytes, stream>>>(A);
-  FPB_CUDA(cudaGetLastError());
-  if (!split) return FPB_OK;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas);
+  int sms = 0;
+  FPB_TRY(sm_count(&sms));
+  cfg.gridDim = dim3(std::min(s.max_ctas, sms * dec_ctas_per_sm(NT)));
+  FPB_CUDA(cudaLaunchKernelEx(&cfg, kernel, A));
   cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
+  cfg.dynamicSmemBytes = 0;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
   cfg.numAttrs = 1;
   FPB_CUDA(cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<T>, A));
   return FPB_OK;
@@ -216,7 +235,7 @@ int fpb_paged_decode(const void* q, int dtype, int batch, int hq, int hk, int he
   FPB_CHECK_ARG((reinterpret_cast<uintptr_t>(lse) & 3) == 0, "lse must be an aligned float pointer or NULL");
   FPB_CHECK_ARG(std::isfinite(sm_scale), "sm_scale must be finite");
   const DecodeShape s = decode_shape(batch, hq, hk, cache_dtype, max_pages, page_size);
-  if (s.split) {
+  if (s.cluster == 0) {
     FPB_CHECK_ARG(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                   "workspace must be a 256-byte aligned device pointer");
     FPB_CHECK_ARG((int64_t)workspace_bytes >= decode_ws_total(s), "workspace too small: %zu bytes given, %lld needed",
@@ -244,17 +263,20 @@ int fpb_paged_decode(const void* q, int dtype, int batch, int hq, int hk, int he
   A.ngroups = s.ngroups;
   A.nh = s.nh;
   A.c = (float)(sm_scale * 1.4426950408889634);
-  int sms = 0;
-  FPB_TRY(sm_count(&sms));
-  const int ctas = std::min(s.max_ctas, sms * kDecCtasPerSm);
+  int log2_page = 0;
+  while ((int64_t(1) << log2_page) < page_size) ++log2_page;
+  // exact for tokens below 2^31: the multiplier exceeds 2^shift / page_size by less than one
+  A.page_shift = 31 + log2_page;
+  A.page_mul = (unsigned)((uint64_t(1) << A.page_shift) / page_size + 1);
+  A.page16 = page_size % 16 == 0;
   auto st = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == FPB_BF16, e4m3 = cache_dtype == FPB_E4M3, wide = s.nh > 8;
   if (bf16) {
-    if (e4m3) return wide ? launch_decode<__nv_bfloat16, true, 2>(A, ctas, s.split, st) : launch_decode<__nv_bfloat16, true, 1>(A, ctas, s.split, st);
-    return wide ? launch_decode<__nv_bfloat16, false, 2>(A, ctas, s.split, st) : launch_decode<__nv_bfloat16, false, 1>(A, ctas, s.split, st);
+    if (e4m3) return wide ? launch_decode<__nv_bfloat16, true, 2>(A, s, st) : launch_decode<__nv_bfloat16, true, 1>(A, s, st);
+    return wide ? launch_decode<__nv_bfloat16, false, 2>(A, s, st) : launch_decode<__nv_bfloat16, false, 1>(A, s, st);
   }
-  if (e4m3) return wide ? launch_decode<__half, true, 2>(A, ctas, s.split, st) : launch_decode<__half, true, 1>(A, ctas, s.split, st);
-  return wide ? launch_decode<__half, false, 2>(A, ctas, s.split, st) : launch_decode<__half, false, 1>(A, ctas, s.split, st);
+  if (e4m3) return wide ? launch_decode<__half, true, 2>(A, s, st) : launch_decode<__half, true, 1>(A, s, st);
+  return wide ? launch_decode<__half, false, 2>(A, s, st) : launch_decode<__half, false, 1>(A, s, st);
 }
 
 int fpb_paged_read_device_error(uint32_t* flags, void* stream) {

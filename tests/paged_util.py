@@ -35,15 +35,15 @@ def quantise(x):
     return (x * (448.0 / amax)).to(E4M3), (amax / 448.0).squeeze(-1)
 
 
-def fill_sequences(lens, hq, hk, dtype, cache_dtype, page_size, layout="hnd", seed=0, spare=2, k_gain=1.0):
+def fill_sequences(lens, hq, hk, dtype, cache_dtype, page_size, layout="hnd", seed=0, spare=2, k_gain=1.0, room=0):
     """Random sequences in pages of mixed order.  Rows that no sequence holds are NaN; table entries behind a sequence point
-    outside the cache.  Returns a dict with the caches, table, lengths, q, and the rows' values in 64 bits."""
+    outside the cache, and the table is wide enough for `room` tokens.  Returns a dict with the caches, table, lengths, q, and the rows' values in 64 bits."""
     g = torch.Generator(device="cuda").manual_seed(seed)
     counts = [-(-n // page_size) for n in lens]
     pages = sum(counts) + spare
     k, v, ks, vs = empty_cache(pages, page_size, hk, cache_dtype, layout)
     order = torch.randperm(pages, generator=g, device="cuda")
-    width = max(max(counts), 1) + 1
+    width = max(max(counts) + 1, -(-room // page_size))
     table = torch.full((len(lens), width), 2 ** 30, dtype=torch.int32, device="cuda")
     rows = []
     used = 0

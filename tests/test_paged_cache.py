@@ -94,8 +94,8 @@ def _decode(lib, **over):
 @pytest.mark.parametrize("over,msg", [
     (dict(hq=7), "multiple"), (dict(hq=0), "multiple"), (dict(b=0), "batch"), (dict(q=8), "q must be 16-byte"), (dict(qs=[1024, 4]), "q stride"),
     (dict(out=0), "out"), (dict(out=1025), "out"), (dict(os=None), "out strides"), (dict(os=[-1, 128]), "out stride[0]"),
-    (dict(lse=1026), "lse"), (dict(scale=float("nan")), "sm_scale"), (dict(ws=0), "workspace"), (dict(ws=4100), "workspace"),
-    (dict(wsb=100), "workspace too small"), (dict(table=0), "page_table"), (dict(lens=2), "seq_lens"), (dict(d=256), "head_dim"),
+    (dict(lse=1026), "lse"), (dict(scale=float("nan")), "sm_scale"), (dict(ws=0, mp=8192), "workspace"), (dict(ws=4100, mp=8192), "workspace"),
+    (dict(wsb=100, mp=8192), "workspace too small"), (dict(table=0), "page_table"), (dict(lens=2), "seq_lens"), (dict(d=256), "head_dim"),
     (dict(cd=1), "16-bit type"), (dict(b=1 << 28), "2^31"),
 ])
 def test_decode_refuses_on_the_host(lib, over, msg):
@@ -105,9 +105,9 @@ def test_decode_refuses_on_the_host(lib, over, msg):
 
 def test_decode_workspace_is_bounded():
     n = fp.paged_decode_workspace_bytes
-    assert n(1, 32, 8, BF16, 4, 16) == 0  # one unit of 64 tokens an item: nothing to join
-    small, large = n(1, 32, 8, BF16, 8, 16), n(256, 32, 8, BF16, 8192, 128)
-    assert 0 < small < large == n(1, 32, 8, BF16, 8192, 128) < 4 << 20  # by the GPU's blocks, not by batch or length
+    assert n(1, 32, 8, BF16, 8, 16) == n(256, 32, 8, BF16, 64, 16) == 0  # short sequences: one cluster an item
+    mid, large = n(1, 1, 1, BF16, 129, 64), n(256, 32, 8, BF16, 8192, 128)
+    assert 0 < mid < large == n(1, 32, 8, BF16, 8192, 128) < 4 << 20  # by the GPU's blocks, not by batch or length
     assert n(1, 128, 8, BF16, 8192, 128) > large  # 16 heads an item
     assert n(0, 32, 8, BF16, 8, 16) == n(1, 7, 2, BF16, 8, 16) == 0
 
@@ -267,6 +267,7 @@ DECODE_CASES = [  # lens, q heads, kv heads, page size, layout
     ([130], 33, 1, 128, "hnd"),       # three groups of 11
     ([6000, 1], 8, 8, 128, "hnd"),
     ([40000], 4, 1, 256, "nhd"),
+    ([20000, 0, 3, 9000, 65, 17001], 8, 2, 64, "hnd"),
     ([100] * 150, 8, 2, 16, "nhd"),
 ]
 
@@ -274,11 +275,13 @@ DECODE_CASES = [  # lens, q heads, kv heads, page size, layout
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("wide", [False, True])  # the table's width decides between clusters and stretches
 @pytest.mark.parametrize("case", range(len(DECODE_CASES)))
-def test_decode_matches_the_definition(case, quant, dtype):
+def test_decode_matches_the_definition(case, wide, quant, dtype):
     lens, hq, hk, ps, layout = DECODE_CASES[case]
     cd = E4M3 if quant else dtype
-    f = pu.fill_sequences(lens, hq, hk, dtype, cd, ps, layout, seed=case)
+    f = pu.fill_sequences(lens, hq, hk, dtype, cd, ps, layout, seed=case, room=70000 if wide else 0)
+    assert not wide or fp.paged_decode_workspace_bytes(len(lens), hq, hk, cd, f["page_table"].shape[1], ps) > 0
     out = torch.full_like(f["q"], float("nan"))
     lse = torch.full((len(lens), hq), float("nan"), device="cuda")
     fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], out, lse, f["k_scale"], f["v_scale"])
@@ -302,7 +305,7 @@ def test_decode_flat_and_peaked_rows(quant, gain):
 @pytest.mark.parametrize("quant", [False, True])
 def test_decode_of_large_bf16_queries(quant):
     """Queries beyond fp16's range (an e4m3 cache is multiplied in fp16) and very small ones."""
-    for mult in (1e6, 1e-8):
+    for mult in (2.0 ** 20, 2.0 ** -27):
         f = pu.fill_sequences([200], 4, 1, BF16, E4M3 if quant else BF16, 16, seed=6)
         f["q"] = f["q"] * mult
         out, lse = torch.empty_like(f["q"]), torch.empty(1, 4, device="cuda")
@@ -335,10 +338,11 @@ def test_decode_without_lse_strided_and_in_place():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("quant", [False, True])
-def test_bad_pages_lengths_and_slots_are_reported_and_skipped(quant):
+@pytest.mark.parametrize("room", [0, 50000])
+def test_bad_pages_lengths_and_slots_are_reported_and_skipped(room, quant):
     dtype = BF16
     cd = E4M3 if quant else dtype
-    f = pu.fill_sequences([200, 90, 64], 8, 2, dtype, cd, 16, seed=9)
+    f = pu.fill_sequences([200, 90, 64], 8, 2, dtype, cd, 16, seed=9, room=room)
     scales = (f["k_scale"], f["v_scale"])
     # a page that is not in the cache: its tokens are left out
     for bad in (-1, f["pages"], 2 ** 31 - 1):
@@ -376,9 +380,10 @@ def test_bad_pages_lengths_and_slots_are_reported_and_skipped(quant):
 
 
 @pytest.mark.gpu
-def test_decode_is_deterministic_and_captured_graphs_serve_other_lengths():
+@pytest.mark.parametrize("room", [0, 100000])
+def test_decode_is_deterministic_and_captured_graphs_serve_other_lengths(room):
     """One capture, replayed for other lengths, tables and queries; a second graph on another stream beside it."""
-    f = pu.fill_sequences([4000, 130, 700, 64], 32, 8, BF16, BF16, 16, seed=10)
+    f = pu.fill_sequences([4000, 130, 700, 64], 32, 8, BF16, BF16, 16, seed=10, room=room)
     q, table, lens = f["q"].clone(), f["page_table"].clone(), f["lens"].clone()
     args = (f["k"], f["v"], table, lens)
     outs = [torch.empty_like(q) for _ in range(2)]
@@ -412,7 +417,7 @@ def test_decode_is_deterministic_and_captured_graphs_serve_other_lengths():
 
 @pytest.mark.gpu
 def test_given_workspace_needs_no_initialisation_and_small_ones_are_refused():
-    f = pu.fill_sequences([3000, 10], 8, 2, FP16, FP16, 16, seed=11)
+    f = pu.fill_sequences([3000, 10], 8, 2, FP16, FP16, 16, seed=11, room=40000)
     n = fp.paged_decode_workspace_bytes(2, 8, 2, FP16, f["page_table"].shape[1], 16)
     args = (f["q"], f["k"], f["v"], f["page_table"], f["lens"])
     want, out = torch.empty_like(f["q"]), torch.empty_like(f["q"])
