@@ -10,10 +10,11 @@
 // An item is (sequence, KV head, group of query heads: all G up to 16, equal groups of at most 16 above that), its tokens are cut
 // into units of kDecWarps * TT.  Lengths are read on the device (no host copy; a captured graph serves any lengths).
 //
-// Long sequences (paged_decode_kernel).  All items' units form one line, and each of a fixed number of CTAs takes an equal stretch
-// of it, so ragged batches and single long sequences load the GPU alike.  A stretch that covers a whole item writes its
-// output; an item cut by a CTA border leaves unnormalised sums and their maxima in the workspace, which a second kernel
-// (programmatic dependent launch) joins in the order of the tokens.
+// Long sequences (paged_decode_kernel).  All items' units form one line, with one empty unit at the head of each item for
+// what starting an item costs, and each of the CTAs that the GPU holds takes an equal piece of it, so ragged batches and
+// single long sequences load the GPU alike.  A piece that covers a whole item writes its output; an item cut between pieces
+// leaves unnormalised sums and their maxima in the workspace, which a second kernel (programmatic dependent launch) joins in
+// the order of the tokens.
 // Short sequences (paged_decode_short_kernel): one cluster of 1 to 8 CTAs for each item, units dealt out in turn, joined
 // through distributed shared memory.  No prefix sums, no workspace, no second kernel.
 // Both join in an order that the lengths alone decide, with no atomics: the same call gives the same bits.
@@ -49,10 +50,9 @@ constexpr int kDecTileBytes = 4096;  // one warp's tile of K or of V
 constexpr int kDecRingBytes = kDecStages * 2 * kDecTileBytes;
 constexpr int kDecSmemBytes = kDecWarps * kDecRingBytes;
 constexpr int dec_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }  // registers: 168 or 255 a thread
-constexpr int kDecMaxCtas = 512;   // bound of the workspace
 constexpr int kDecMaxCluster = 8;
 static_assert(kDecThreads == kHeadDim, "one thread for each channel in the merges");
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 256;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct DecodeArgs {
@@ -69,9 +69,11 @@ struct DecodeArgs {
   int max_pages, batch, hq, hk;
   int G, ngroups, nh;                // query heads of a KV head, groups of them, heads of a group (the last may have fewer)
   float c;                           // sm_scale * log2(e)
-  int4* desc;                        // per CTA: {b, KV head * groups + group, partials, 0} of the item it begins and does not end
-  float* part;                       // [2 * CTA + slot][nh][128]
-  float2* ml;                        // [2 * CTA + slot][nh] {maximum (log2 units), sum}
+  int by_item;                       // desc is indexed by item (else by the piece that begins the item)
+  int join_heads;                    // heads of a CTA of the second kernel
+  int4* desc;                        // {b, KV head * groups + group, first piece, pieces (0: nothing to join)}
+  float* part;                       // [2 * piece + slot][nh][128]; slot 1 where the piece begins the item, else 0
+  float2* ml;                        // [2 * piece + slot][nh] {maximum (log2 units), sum}
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -154,45 +156,50 @@ struct DecodeWarp {
   float m[NT][2], l[NT][2];   // running maximum and this thread's share of the sum
   float vref, vinv;           // e4m3: largest V scale so far and its reciprocal
 
+  // q's rows as they are in memory.  An e4m3 row gives a thread elements 4t .. 4t+3 of each 16: they take the places 2t,
+  // 2t+1, 2t+8, 2t+9 of the product's inner dimension, in q as in K.
   __device__ __forceinline__ void load_q(const DecodeArgs& A, const uint8_t* q, int heads) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const bool ok = n * 8 + g < heads;
       const uint8_t* row = q + (n * 8 + g) * A.q_h;
-      float f = 1.f;
-      if constexpr (!kE4m3) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 8; ++k) {
+        if constexpr (!kE4m3) {
           qf[n][k][0] = ok ? __ldg(reinterpret_cast<const uint32_t*>(row + 32 * k + 4 * t)) : 0u;
           qf[n][k][1] = ok ? __ldg(reinterpret_cast<const uint32_t*>(row + 32 * k + 4 * t + 16)) : 0u;
-        }
-      } else {
-        // an e4m3 row gives a thread elements 4t .. 4t+3 of each 16: they take the places 2t, 2t+1, 2t+8, 2t+9 of the
-        // product's inner dimension, in q as in K
-        uint32_t mx = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        } else {
           const uint2 x = ok ? __ldg(reinterpret_cast<const uint2*>(row + 32 * k + 8 * t)) : make_uint2(0u, 0u);
           qf[n][k][0] = x.x;
           qf[n][k][1] = x.y;
-          mx = absmax2(absmax2(mx, x.x), x.y);
         }
-        if constexpr (DT<T>::is_bf16) {
-          mx = max(mx & 0xFFFFu, mx >> 16);
-          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          // power of two that brings the row's largest magnitude to [1, 2); inf and NaN pass as they are
-          int e = (int)(mx >> 7) - 127;
-          e = max(-120, min(e, 120));
-          const float down = exp2i(-e);
-          f = exp2i(e);
+      }
+    }
+  }
+  // q in the products' type and the factors of the scores.
+  __device__ __forceinline__ void convert_q(const DecodeArgs& A) {
+    const int t = lane & 3;
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
+    for (int n = 0; n < NT; ++n) {
+      float f = 1.f;
+      if constexpr (kE4m3 && DT<T>::is_bf16) {
+        uint32_t mx = 0;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              qf[n][k][j] = DT<__half>::pack(DT<T>::lo(qf[n][k][j]) * down, DT<T>::hi(qf[n][k][j]) * down);
-        }
+        for (int k = 0; k < 8; ++k) mx = absmax2(absmax2(mx, qf[n][k][0]), qf[n][k][1]);
+        mx = max(mx & 0xFFFFu, mx >> 16);
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // power of two that brings the row's largest magnitude to [1, 2); inf and NaN pass as they are
+        int e = (int)(mx >> 7) - 127;
+        e = max(-120, min(e, 120));
+        const float down = exp2i(-e);
+        f = exp2i(e);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            qf[n][k][j] = DT<__half>::pack(DT<T>::lo(qf[n][k][j]) * down, DT<T>::hi(qf[n][k][j]) * down);
       }
       qc[n][0] = A.c * __shfl_sync(0xffffffffu, f, 8 * t);
       qc[n][1] = A.c * __shfl_sync(0xffffffffu, f, 8 * t + 4);
@@ -461,7 +468,6 @@ struct DecodeWarp {
     int page[MTILES];
     load_pages(A, table, tok, page);
     load_q(A, A.q + b * A.q_b + head0 * A.q_h, heads);
-    reset();
     const int n = end > tok ? (end - tok + step - 1) / step : 0;
     uint32_t valid[kDecStages];
     float ks[kDecStages], vs[kDecStages];
@@ -476,6 +482,8 @@ struct DecodeWarp {
       }
       cp_async_commit();
     }
+    convert_q(A);
+    reset();
     for (int i0 = 0; i0 < n; i0 += kDecStages) {
 #pragma unroll
       for (int j = 0; j < kDecStages; ++j) {
@@ -547,66 +555,65 @@ __device__ __forceinline__ void write_head(const DecodeArgs& A, int b, int head,
   if (A.lse && tid == 0) A.lse[(int64_t)b * A.hq + head] = l == 0.f ? -INFINITY : (mx + log2f(l)) * kLn2;
 }
 
+// Equal cuts of `total` units into `n` pieces: piece i starts at i * q + min(i, r).
+struct Cut {
+  int q, r;
+  __device__ __forceinline__ Cut(int total, int n) : q(total / n), r(total - q * n) {}
+  __device__ __forceinline__ int start(int i) const { return i * q + min(i, r); }
+  __device__ __forceinline__ int piece(int t) const { return t < r * (q + 1) ? t / (q + 1) : r + (t - r * (q + 1)) / q; }
+};
+
 template <typename T, bool kE4m3, int NT>
 __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode_kernel(const DecodeArgs A) {
   using W = DecodeWarp<T, kE4m3, NT>;
   constexpr int kUnit = kDecWarps * W::TT;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 s_ml[kDecWarps][8 * NT];
-  __shared__ int64_t s_scan[kDecWarps];
-  __shared__ int64_t s_start[2];
   static_assert(8 * NT * 132 * 4 <= kDecRingBytes, "a warp's sums fit its ring");
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int HH = A.hk * A.ngroups;
+  const int HH = A.hk * A.ngroups, v = blockIdx.x;
 
-  // ---- this CTA's stretch: prefix sums of the sequences' units (a sequence without tokens has one, empty)
-  const int per = (A.batch + kDecThreads - 1) / kDecThreads;
-  const int b_lo = min(tid * per, A.batch), b_hi = min(b_lo + per, A.batch);
-  int64_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += max(1, (seq_len_of(A, b) + kUnit - 1) / kUnit);
-  int64_t incl = mine;
+  // ---- this CTA's piece, found by every warp for itself: prefix sums of the sequences' units.  The host has checked that
+  // all units together stay below 2^31.
+  auto units_of = [](int len) { return 1 + (len + kUnit - 1) / kUnit; };
+  const int per = (A.batch + 31) / 32;
+  const int b_lo = min(lane * per, A.batch), b_hi = min(b_lo + per, A.batch);
+  int mine = 0;
+#pragma unroll 8
+  for (int i = b_lo; i < b_hi; ++i) mine += units_of(seq_len_of(A, i));
+  int incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, incl, d);
+    const int x = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += x;
   }
-  if (lane == 31) s_scan[warp] = incl;
-  __syncthreads();
-  int64_t total = 0, before = 0;
-#pragma unroll
-  for (int w = 0; w < kDecWarps; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
-  }
-  incl += before;
-  total *= HH;
-  const int64_t ctas = min((int64_t)gridDim.x, total);
-  if (tid == 0) A.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
-  if ((int64_t)blockIdx.x >= ctas) return;
-  int64_t t = (int64_t)blockIdx.x * total / ctas;
-  const int64_t t_end = ((int64_t)blockIdx.x + 1) * total / ctas;
-  {
-    int64_t base = (incl - mine) * HH;
-    if (base <= t && t < incl * HH) {  // one thread
-      int b = b_lo;
-      while (true) {
-        const int64_t n = (int64_t)max(1, (seq_len_of(A, b) + kUnit - 1) / kUnit) * HH;
-        if (t < base + n) break;
-        base += n;
-        ++b;
-      }
-      s_start[0] = b;
-      s_start[1] = base;
+  const int total = __shfl_sync(0xffffffffu, incl, 31) * HH;
+  const int pieces = min((int)gridDim.x, total);
+  if (!A.by_item && tid == 0) A.desc[v] = make_int4(0, 0, 0, 0);
+  if (v >= pieces) return;
+  const Cut cut(total, pieces);
+  int t = cut.start(v);
+  const int t_end = cut.start(v + 1);
+  int b = b_lo, len = 0, base = (incl - mine) * HH;
+  const bool here = base <= t && t < incl * HH;  // one lane
+  if (here) {
+    while (true) {
+      len = seq_len_of(A, b);
+      const int n = units_of(len) * HH;
+      if (t < base + n) break;
+      base += n;
+      ++b;
     }
   }
-  __syncthreads();
-  int b = (int)s_start[0];
-  int len = seq_len_of(A, b);
-  int units = max(1, (len + kUnit - 1) / kUnit);
-  int hh = (int)((t - s_start[1]) / units);
-  int u = (int)((t - s_start[1]) - (int64_t)hh * units);
+  const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  b = __shfl_sync(0xffffffffu, b, src);
+  len = __shfl_sync(0xffffffffu, len, src);
+  base = __shfl_sync(0xffffffffu, base, src);
+  int units = units_of(len);
+  int hh = (t - base) / units;
+  int u = (t - base) - hh * units;
 
   W w;
   w.lane = lane;
@@ -614,29 +621,30 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
   float* const so = reinterpret_cast<float*>(smem + warp * kDecRingBytes);
 
   while (t < t_end) {
-    const int u_end = (int)min((int64_t)units, u + (t_end - t));
+    const int u_end = min(units, u + (t_end - t));
     const int h = hh / A.ngroups, grp = hh - h * A.ngroups;
     const int head0 = h * A.G + grp * A.nh, heads = min(A.nh, A.G - grp * A.nh);
-    w.run(A, b, h * A.C.s_head, h * A.C.ss_head, head0, heads, u * kUnit + warp * W::TT, kUnit, min(len, u_end * kUnit));
+    // units u .. u_end hold the tokens [(u - 1) kUnit, (u_end - 1) kUnit); the first of an item none
+    w.run(A, b, h * A.C.s_head, h * A.C.ss_head, head0, heads, max(u - 1, 0) * kUnit + warp * W::TT, kUnit,
+          min(len, (u_end - 1) * kUnit));
     w.store(so, s_ml[warp]);
     __syncthreads();
 
     const bool whole = u == 0 && u_end == units;
-    const int slot = 2 * blockIdx.x + (u == 0 ? 1 : 0);
+    const int64_t slot = 2 * v + (u == 0 ? 1 : 0);
     for (int i = 0; i < heads; ++i) {
       float x, l, mx;
       merge_warps<NT>(smem, s_ml, i, tid, x, l, mx);
       if (whole) {
         write_head<T>(A, b, head0 + i, tid, x, l, mx);
       } else {
-        A.part[((int64_t)slot * A.nh + i) * kHeadDim + tid] = x;
-        if (tid == 0) A.ml[(int64_t)slot * A.nh + i] = make_float2(mx, l);
+        A.part[(slot * A.nh + i) * kHeadDim + tid] = x;
+        if (tid == 0) A.ml[slot * A.nh + i] = make_float2(mx, l);
       }
     }
-    if (!whole && u == 0 && tid == 0) {
-      const int64_t last = t + units - 1;  // unit of the item's end; its CTA
-      const int64_t c1 = ((last + 1) * ctas - 1) / total;
-      A.desc[blockIdx.x] = make_int4(b, hh, (int)(c1 - blockIdx.x) + 1, 0);
+    if (u == 0 && tid == 0 && (A.by_item || !whole)) {
+      const int v1 = cut.piece(t + units - 1);  // of the item's last unit
+      A.desc[A.by_item ? b * HH + hh : v] = make_int4(b, hh, v, v1 > v ? v1 - v + 1 : 0);
     }
     __syncthreads();
 
@@ -646,7 +654,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
       hh = 0;
       if (++b < A.batch) {
         len = seq_len_of(A, b);
-        units = max(1, (len + kUnit - 1) / kUnit);
+        units = units_of(len);
       }
     }
   }
@@ -712,70 +720,81 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
   cluster_sync();  // no CTA leaves while others read its sums
 }
 
-// Joins the partial sums of the item that CTA blockIdx.x of the first kernel began and did not end.  A warp takes one head
-// and every parts-th partial (all maxima first, then the weighted sums, four channels a lane); the parts meet in shared
-// memory.  What the first loads need does not depend on the description, so they travel together.
+__device__ __forceinline__ void scale4(float4& x, float f) { x = make_float4(x.x * f, x.y * f, x.z * f, x.w * f); }
+__device__ __forceinline__ void add4(float4& x, float f, const float4& p) {
+  x.x += f * p.x;
+  x.y += f * p.y;
+  x.z += f * p.z;
+  x.w += f * p.w;
+}
+
+// Joins the pieces of the item of desc[blockIdx.x], heads [blockIdx.y * join_heads, + join_heads).  A warp takes one head and
+// every parts-th piece, four of them and their maxima under way at a time; the parts meet in shared memory.
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_decode_join_kernel(const DecodeArgs A) {
   constexpr int kWarps = kJoinThreads / 32;
   __shared__ float s_x[kWarps][kHeadDim];
-  __shared__ float s_l[kWarps];
+  __shared__ float2 s_ml[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int parts = kWarps / A.nh;  // nh <= 16
-  const int i = warp % A.nh, part = warp / A.nh;
-  const int room = gridDim.x - blockIdx.x;
-  auto slot = [&](int k) { return (int64_t)(2 * (blockIdx.x + k) + (k == 0 ? 1 : 0)) * A.nh + i; };
-  auto sums = [&](int k) { return reinterpret_cast<const float4*>(A.part + slot(k) * kHeadDim)[lane]; };
+  const int parts = kWarps / A.join_heads;  // join_heads <= kWarps
+  const int part = warp / A.join_heads, i = blockIdx.y * A.join_heads + warp % A.join_heads;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 d = A.desc[blockIdx.x];
-  const float2 early = lane < room ? A.ml[slot(lane)] : make_float2(-INFINITY, 0.f);
-  const float4 first = part < min(parts, room) ? sums(part) : make_float4(0.f, 0.f, 0.f, 0.f);
-  const int n = d.z;
+  const int n = d.w;
   if (n == 0) return;
   const int b = d.x, h = d.y / A.ngroups, grp = d.y - h * A.ngroups;
   const int head0 = h * A.G + grp * A.nh, heads = min(A.nh, A.G - grp * A.nh);
+  auto slot = [&](int k) { return (int64_t)(2 * (d.z + k) + (k == 0 ? 1 : 0)) * A.nh + i; };
   const bool mine = part < parts && i < heads;
-  float mx = lane < n ? early.x : -INFINITY;
-  for (int k = lane + 32; k < n; k += 32) mx = fmaxf(mx, A.ml[slot(k)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const float ref = finite_or_zero(mx);
+  float mx = -INFINITY, l = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
   if (mine) {
-#pragma unroll 8
-    for (int k = part; k < n; k += parts) {
-      const float em = __shfl_sync(0xffffffffu, early.x, k & 31), el = __shfl_sync(0xffffffffu, early.y, k & 31);
-      const float2 ml = k < 32 ? make_float2(em, el) : A.ml[slot(k)];
-      const float4 p = k == part ? first : sums(k);
-      const float f = ex2_approx(ml.x - ref);
-      l += f * ml.y;
-      x.x += f * p.x;
-      x.y += f * p.y;
-      x.z += f * p.z;
-      x.w += f * p.w;
+    constexpr int kBatch = 4;
+    for (int k0 = part; k0 < n; k0 += kBatch * parts) {
+      float2 ml[kBatch];
+      float4 p[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int k = k0 + j * parts;
+        ml[j] = k < n ? A.ml[slot(k)] : make_float2(-INFINITY, 0.f);
+        p[j] = k < n ? reinterpret_cast<const float4*>(A.part + slot(k) * kHeadDim)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float top = mx;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) top = fmaxf(top, ml[j].x);
+      const float ref = finite_or_zero(top), f0 = ex2_approx(mx - ref);
+      mx = top;
+      l *= f0;
+      scale4(x, f0);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const float f = ex2_approx(ml[j].x - ref);
+        l += f * ml[j].y;
+        add4(x, f, p[j]);
+      }
     }
     reinterpret_cast<float4*>(s_x[warp])[lane] = x;
-    if (lane == 0) s_l[warp] = l;
+    if (lane == 0) s_ml[warp] = make_float2(mx, l);
   }
   __syncthreads();
   if (!mine || part != 0) return;
+  float top = mx;
+  for (int k = 1; k < parts; ++k) top = fmaxf(top, s_ml[warp + k * A.join_heads].x);
+  const float ref = finite_or_zero(top), f0 = ex2_approx(mx - ref);
+  mx = top;
+  l *= f0;
+  scale4(x, f0);
   for (int k = 1; k < parts; ++k) {
-    const float4 p = reinterpret_cast<const float4*>(s_x[warp + k * A.nh])[lane];
-    l += s_l[warp + k * A.nh];
-    x.x += p.x;
-    x.y += p.y;
-    x.z += p.z;
-    x.w += p.w;
+    const float2 ml = s_ml[warp + k * A.join_heads];
+    const float f = ex2_approx(ml.x - ref);
+    l += f * ml.y;
+    add4(x, f, reinterpret_cast<const float4*>(s_x[warp + k * A.join_heads])[lane]);
   }
-  const float inv = 1.f / l;
-  if (l == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float f = l == 0.f ? 0.f : inv;
   T* out = reinterpret_cast<T*>(A.out + b * A.o_b + (head0 + i) * A.o_h) + 4 * lane;
-  out[0] = DT<T>::from_f(x.x * f);
-  out[1] = DT<T>::from_f(x.y * f);
-  out[2] = DT<T>::from_f(x.z * f);
-  out[3] = DT<T>::from_f(x.w * f);
+  out[0] = DT<T>::from_f(l == 0.f ? 0.f : x.x / l);
+  out[1] = DT<T>::from_f(l == 0.f ? 0.f : x.y / l);
+  out[2] = DT<T>::from_f(l == 0.f ? 0.f : x.z / l);
+  out[3] = DT<T>::from_f(l == 0.f ? 0.f : x.w / l);
   if (A.lse && lane == 0) A.lse[(int64_t)b * A.hq + head0 + i] = l == 0.f ? -INFINITY : (mx + log2f(l)) * kLn2;
 }
 

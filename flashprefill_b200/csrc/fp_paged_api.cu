@@ -68,32 +68,42 @@ void head_groups(int G, int* ngroups, int* nh) {
 }
 
 // How a call runs.  Short sequences: clusters of the least power of two of CTAs that fills the GPU's places (at most 8, and
-// no more than an item can have units), if that leaves at most kShortUnits units to a CTA; else equal stretches of all units.
+// no more than an item can have units), if that leaves at most kShortUnits units to a CTA; else pieces of the line of all
+// units.  Every size here is a bound from the table's width: lengths are known on the device only.
 constexpr int kShortUnits = 16;
-constexpr int kDecPlaces = 148 * 3;
 struct DecodeShape {
-  int G, ngroups, nh, max_ctas, cluster;  // cluster: 0 for stretches
-  int64_t items;
+  int G, ngroups, nh;
+  int cluster;           // 0: pieces
+  int pieces;            // CTAs: the places of a 148-SM GPU
+  int by_item, join_heads;
+  int64_t items, units;  // all items; all units at most
 };
 DecodeShape decode_shape(int batch, int hq, int hk, int cache_dtype, int max_pages, int page_size) {
   DecodeShape s{};
   s.G = hq / hk;
   head_groups(s.G, &s.ngroups, &s.nh);
   const int unit = kDecWarps * (cache_dtype == FPB_E4M3 ? 32 : 16);
+  const int places = 148 * dec_ctas_per_sm(s.nh <= 8 ? 1 : 2);
   const int64_t units = ((int64_t)max_pages * page_size + unit - 1) / unit;
   s.items = (int64_t)batch * hk * s.ngroups;
+  s.units = s.items * (units + 1);
   int cluster = 1;
-  while (cluster < kDecMaxCluster && 2 * cluster <= units && s.items * cluster < kDecPlaces) cluster *= 2;
+  while (cluster < kDecMaxCluster && 2 * cluster <= units && s.items * cluster < places) cluster *= 2;
   s.cluster = (units + cluster - 1) / cluster <= kShortUnits && s.items * cluster < (int64_t(1) << 31) ? cluster : 0;
-  s.max_ctas = (int)std::min<int64_t>(kDecMaxCtas, units >= kDecMaxCtas ? kDecMaxCtas : s.items * units);
+  s.pieces = (int)std::min<int64_t>(places, s.units);
+  s.by_item = s.items <= s.pieces;
+  // heads share a CTA of the join where an item has few pieces, and have one each where it has many
+  const int64_t each = s.pieces / s.items;
+  s.join_heads = each >= 16 ? 1 : each >= 4 ? 2 : std::min(s.nh, kJoinThreads / 32);
   return s;
 }
-int64_t decode_ws_part(const DecodeShape& s) { return align256(16 * (int64_t)s.max_ctas); }
+int decode_descs(const DecodeShape& s) { return s.by_item ? (int)s.items : s.pieces; }
+int64_t decode_ws_part(const DecodeShape& s) { return align256(16 * (int64_t)decode_descs(s)); }
 int64_t decode_ws_ml(const DecodeShape& s) {
-  return decode_ws_part(s) + align256(2 * (int64_t)s.max_ctas * s.nh * kHeadDim * 4);
+  return decode_ws_part(s) + align256(2 * (int64_t)s.pieces * s.nh * kHeadDim * 4);
 }
 int64_t decode_ws_total(const DecodeShape& s) {
-  return s.cluster ? 0 : decode_ws_ml(s) + align256(2 * (int64_t)s.max_ctas * s.nh * 8);
+  return s.cluster ? 0 : decode_ws_ml(s) + align256(2 * (int64_t)s.pieces * s.nh * 8);
 }
 
 template <typename T, bool kE4m3, int NT>
@@ -117,10 +127,9 @@ int launch_decode(const DecodeArgs& A, const DecodeShape& s, cudaStream_t stream
   }
   auto kernel = paged_decode_kernel<T, kE4m3, NT>;
   FPB_TRY(set_smem(kernel, kDecSmemBytes));
-  int sms = 0;
-  FPB_TRY(sm_count(&sms));
-  cfg.gridDim = dim3(std::min(s.max_ctas, sms * dec_ctas_per_sm(NT)));
+  cfg.gridDim = dim3(s.pieces);
   FPB_CUDA(cudaLaunchKernelEx(&cfg, kernel, A));
+  cfg.gridDim = dim3(decode_descs(s), (s.nh + s.join_heads - 1) / s.join_heads);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -236,6 +245,7 @@ int fpb_paged_decode(const void* q, int dtype, int batch, int hq, int hk, int he
   FPB_CHECK_ARG(std::isfinite(sm_scale), "sm_scale must be finite");
   const DecodeShape s = decode_shape(batch, hq, hk, cache_dtype, max_pages, page_size);
   if (s.cluster == 0) {
+    FPB_CHECK_ARG(s.units < (int64_t(1) << 31), "too many tokens for one call: batch * num_kv_heads * max_pages * page_size (narrow the page table)");
     FPB_CHECK_ARG(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                   "workspace must be a 256-byte aligned device pointer");
     FPB_CHECK_ARG((int64_t)workspace_bytes >= decode_ws_total(s), "workspace too small: %zu bytes given, %lld needed",
@@ -262,6 +272,8 @@ int fpb_paged_decode(const void* q, int dtype, int batch, int hq, int hk, int he
   A.G = s.G;
   A.ngroups = s.ngroups;
   A.nh = s.nh;
+  A.by_item = s.by_item;
+  A.join_heads = s.join_heads;
   A.c = (float)(sm_scale * 1.4426950408889634);
   int log2_page = 0;
   while ((int64_t(1) << log2_page) < page_size) ++log2_page;
