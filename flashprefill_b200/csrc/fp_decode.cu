@@ -64,8 +64,7 @@ struct DecodeArgs {
   const int* page_table;
   int64_t table_stride;
   const int* seq_lens;
-  unsigned page_mul;                 // token / page_size = token * page_mul >> page_shift
-  int page_shift, page16;            // page16: page_size is a multiple of 16
+  int page16;                        // page_size is a multiple of 16
   int max_pages, batch, hq, hk;
   int G, ngroups, nh;                // query heads of a KV head, groups of them, heads of a group (the last may have fewer)
   float c;                           // sm_scale * log2(e)
@@ -130,10 +129,6 @@ __device__ __forceinline__ int seq_len_of(const DecodeArgs& A, int b) {
     return 0;
   }
   return len;
-}
-
-__device__ __forceinline__ int page_of(const DecodeArgs& A, int tok) {
-  return (int)(((uint64_t)(unsigned)tok * A.page_mul) >> A.page_shift);
 }
 
 // T: type of q and out; kE4m3: codes in the cache (else T); NT: groups of 8 heads of an item.
@@ -224,15 +219,15 @@ struct DecodeWarp {
   __device__ __forceinline__ void load_pages(const DecodeArgs& A, const int* table, int tok, int (&page)[MTILES]) {
 #pragma unroll
     for (int j = 0; j < MTILES; ++j) {
-      const int p = page_of(A, tok + 16 * j);
+      const int p = A.C.page_of(tok + 16 * j);
       page[j] = p < A.max_pages ? __ldg(table + p) : -1;
     }
   }
 
   // Starts the copies of tokens [tok, tok + TT) below `end` into ring slot `stage`.  valid: bit r set where row r is there;
   // ks, vs: the scales of this lane's token.
-  __device__ __forceinline__ void issue(const DecodeArgs& A, const int* table, int64_t head_off, int64_t scale_off, int tok,
-                                        int end, int stage, const int (&page)[MTILES], uint32_t& valid, float& ks, float& vs) {
+  __device__ __forceinline__ void issue(const DecodeArgs& A, const int* table, int h, int tok, int end,
+                                        int stage, const int (&page)[MTILES], uint32_t& valid, float& ks, float& vs) {
     constexpr int kRowsPer = 32 / kChunks;  // rows of one copy instruction of the warp
     const uint32_t kd = ring + stage * 2 * kDecTileBytes, vd = kd + kDecTileBytes;
     const int ch = lane % kChunks, r0 = lane / kChunks;
@@ -243,18 +238,18 @@ struct DecodeWarp {
       for (int j = 0; j < MTILES; ++j) {
         const int t0 = tok + 16 * j;
         int rows = max(0, min(16, end - t0));
-        int64_t pg = page[j];
-        if (rows > 0 && (unsigned)page[j] >= (unsigned)A.C.num_pages) {
+        unsigned pg = page[j];
+        if (rows > 0 && pg >= (unsigned)A.C.num_pages) {
           raise_error(&g_paged_err, kErrBadPage);
           rows = 0;
         }
         if (rows == 0) pg = 0;
-        const int at = rows == 0 ? 0 : t0 - page_of(A, t0) * A.C.page_size;
+        const int at = rows == 0 ? 0 : t0 - A.C.page_of(t0) * A.C.page_size;
         valid |= ((1u << rows) - 1u) << (16 * j);
-        const int64_t off = pg * A.C.s_page + (int64_t)(at + r0) * A.C.s_tok + head_off + ch * 16;
+        const uint64_t off = A.C.rows.at(pg, at + r0, h) * 16 + ch * 16;
         const uint8_t* kp = A.C.k + off;
         const uint8_t* vp = A.C.v + off;
-        const int64_t step = kRowsPer * A.C.s_tok;
+        const uint64_t step = (uint64_t)A.C.rows.tok * (16 * kRowsPer);
 #pragma unroll
         for (int i = 0; i < 16 / kRowsPer; ++i) {
           const int r = i * kRowsPer + r0, row = 16 * j + r;
@@ -267,7 +262,7 @@ struct DecodeWarp {
         }
         if constexpr (kE4m3) {
           if (lane / 16 == j && lane % 16 < rows) {
-            const int64_t so = pg * A.C.ss_page + (int64_t)(at + lane % 16) * A.C.ss_tok + scale_off;
+            const uint64_t so = A.C.scales.at(pg, at + lane % 16, h);
             ks = __ldg(A.C.k_scale + so);
             vs = __ldg(A.C.v_scale + so);
           }
@@ -278,11 +273,11 @@ struct DecodeWarp {
     const int my = tok + lane % TT;
     int64_t off = -1;
     if (my < end) {
-      const int p = page_of(A, my), at = my - p * A.C.page_size, pg = __ldg(table + p);
+      const int p = A.C.page_of(my), at = my - p * A.C.page_size, pg = __ldg(table + p);
       if ((unsigned)pg < (unsigned)A.C.num_pages) {
-        off = (int64_t)pg * A.C.s_page + (int64_t)at * A.C.s_tok;
+        off = (int64_t)(A.C.rows.at(pg, at, h) * 16);
         if constexpr (kE4m3) {
-          const int64_t so = (int64_t)pg * A.C.ss_page + (int64_t)at * A.C.ss_tok + scale_off;
+          const uint64_t so = A.C.scales.at(pg, at, h);
           ks = __ldg(A.C.k_scale + so);
           vs = __ldg(A.C.v_scale + so);
         }
@@ -297,7 +292,7 @@ struct DecodeWarp {
       const int r = i * kRowsPer + r0;
       const int64_t ro = __shfl_sync(0xffffffffu, off, r);
       const uint32_t d = r * kRowBytes + ((ch ^ (r & 7)) << 4);
-      const int64_t so = ro < 0 ? 0 : ro + head_off + ch * 16;
+      const int64_t so = ro < 0 ? 0 : ro + ch * 16;
       cp_async16(kd + d, A.C.k + so, ro < 0 ? 0 : 16);
       cp_async16(vd + d, A.C.v + so, ro < 0 ? 0 : 16);
     }
@@ -462,8 +457,7 @@ struct DecodeWarp {
 
   // All of this warp's tiles of an item: tokens [tok + i * step, + TT) below min(end, the sequence's length).  The first
   // table entries and q are on their way before the length is needed.
-  __device__ __forceinline__ void run(const DecodeArgs& A, int b, int64_t head_off, int64_t scale_off, int head0, int heads,
-                                      int tok, int step, int end) {
+  __device__ __forceinline__ void run(const DecodeArgs& A, int b, int h, int head0, int heads, int tok, int step, int end) {
     const int* table = A.page_table + b * A.table_stride;
     int page[MTILES];
     load_pages(A, table, tok, page);
@@ -478,7 +472,7 @@ struct DecodeWarp {
 #pragma unroll
         for (int j = 0; j < MTILES; ++j) cur[j] = page[j];
         if (i + 1 < n) load_pages(A, table, tok + (i + 1) * step, page);
-        issue(A, table, head_off, scale_off, tok + i * step, end, i, cur, valid[i], ks[i], vs[i]);
+        issue(A, table, h, tok + i * step, end, i, cur, valid[i], ks[i], vs[i]);
       }
       cp_async_commit();
     }
@@ -497,7 +491,7 @@ struct DecodeWarp {
 #pragma unroll
             for (int x = 0; x < MTILES; ++x) cur[x] = page[x];
             if (nx + 1 < n) load_pages(A, table, tok + (nx + 1) * step, page);
-            issue(A, table, head_off, scale_off, tok + nx * step, end, st, cur, valid[st], ks[st], vs[st]);
+            issue(A, table, h, tok + nx * step, end, st, cur, valid[st], ks[st], vs[st]);
           }
           cp_async_commit();
           consume(j, valid[j], ks[j], vs[j]);
@@ -625,7 +619,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
     const int h = hh / A.ngroups, grp = hh - h * A.ngroups;
     const int head0 = h * A.G + grp * A.nh, heads = min(A.nh, A.G - grp * A.nh);
     // units u .. u_end hold the tokens [(u - 1) kUnit, (u_end - 1) kUnit); the first of an item none
-    w.run(A, b, h * A.C.s_head, h * A.C.ss_head, head0, heads, max(u - 1, 0) * kUnit + warp * W::TT, kUnit,
+    w.run(A, b, h, head0, heads, max(u - 1, 0) * kUnit + warp * W::TT, kUnit,
           min(len, (u_end - 1) * kUnit));
     w.store(so, s_ml[warp]);
     __syncthreads();
@@ -677,7 +671,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
   W w;
   w.lane = lane;
   w.ring = smem_u32(smem) + warp * kDecRingBytes;
-  w.run(A, b, h * A.C.s_head, h * A.C.ss_head, head0, heads, rank * kUnit + warp * W::TT, cluster * kUnit, seq_len_of(A, b));
+  w.run(A, b, h, head0, heads, rank * kUnit + warp * W::TT, cluster * kUnit, seq_len_of(A, b));
   w.store(reinterpret_cast<float*>(smem + warp * kDecRingBytes), s_ml[warp]);
   __syncthreads();
   for (int i = 0; i < heads; ++i) {

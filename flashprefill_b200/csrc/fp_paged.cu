@@ -10,9 +10,12 @@
 // and NaN on top, so a row that holds either gets a scale of inf or NaN and reads back as NaN throughout (fmaxf would drop
 // the NaN).  The rounding to e4m3 is the purpose of the type: half the bytes, an error of at most 2^-4 of each value.
 //
-// Both kernels are bound by HBM: each byte moves once, in 16-byte pieces, and one (token, head) row of K and of V is the
-// work of 16 lanes (16-bit cache) or 8 lanes (e4m3: 16 elements a lane, so that amax takes three shuffles and the codes of
-// a lane are one 16-byte store).
+// Both kernels are bound by HBM: each byte moves once, a (token, head) row of K and of V by a group of lanes.  Reading and
+// copying take 16 lanes of 16 bytes a row; quantising takes 8 lanes of 16 elements, because the work of a row that does not
+// shrink with its elements (amax over the lanes, the division, the addresses) would bound it with 16 lanes (131072 tokens of
+// 8 heads, bf16 to e4m3: 177 us against 131).  Where a read is large enough to fill the
+// GPU all the same and 4 divides page_size, the lanes take 4 tokens of a head: one table entry and one division for all, and
+// their loads under way together.
 #include "fp_common.cuh"
 
 namespace fpb {
@@ -25,12 +28,27 @@ enum : uint32_t {
   kErrBadLength = 1u << 5,  // a sequence length outside [0, room]
 };
 
+// x / d for 0 <= x < 2^31: mul exceeds 2^shift / d by at most one, shift = 31 + ceil(log2 d).
+struct FastDiv {
+  unsigned mul;
+  int shift;
+  __device__ __forceinline__ unsigned operator()(unsigned x) const { return (unsigned)(((uint64_t)x * mul) >> shift); }
+};
+
+// Element (a, token, head) of a tensor whose three strides are in 16-byte pieces (rows) or in elements (scales).
+struct Pitch {
+  unsigned outer, tok, head;
+  __device__ __forceinline__ uint64_t at(unsigned a, unsigned t, unsigned h) const {
+    return (uint64_t)a * outer + (uint64_t)t * tok + (uint64_t)h * head;
+  }
+};
+
 struct PagedCache {
-  uint8_t *k, *v;             // codes or 16-bit values
-  float *k_scale, *v_scale;   // e4m3 only
-  int64_t s_page, s_tok, s_head;     // bytes
-  int64_t ss_page, ss_tok, ss_head;  // scale strides in elements
+  uint8_t *k, *v;            // codes or 16-bit values
+  float *k_scale, *v_scale;  // e4m3 only
+  Pitch rows, scales;        // outer: page
   int num_pages, page_size;
+  FastDiv page_of;           // token -> index into its sequence's table; slot -> page
 };
 
 // Longest sequence: token indices and their rounding up to whole tiles stay in 32 bits.
@@ -44,9 +62,18 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)two));
   return r;
 }
-__device__ __forceinline__ uint32_t f32x2_to_e4m3x2(float lo, float hi) {
+// (a0, a1) * b, two products in one instruction
+__device__ __forceinline__ float2 mul2(float a0, float a1, float b) {
+  float2 d;
+  asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %4};\n mul.rn.f32x2 rd, ra, rb;\n"
+      " mov.b64 {%0, %1}, rd;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a0), "f"(a1), "f"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t f32x2_to_e4m3x2(float2 x) {
   unsigned short r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(x.y), "f"(x.x));
   return r;
 }
 
@@ -59,10 +86,11 @@ __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) 
 struct KvWriteArgs {
   PagedCache C;
   const uint8_t *k, *v;
-  int64_t ks_tok, ks_head, vs_tok, vs_head;  // bytes
+  Pitch kp, vp;  // outer unused
   const void* slots;
   int slots64;
   unsigned rows, hk;  // tokens * kv heads
+  FastDiv token_of;   // row -> token
 };
 
 __device__ __forceinline__ int64_t load_slot(const KvWriteArgs& A, unsigned tok) {
@@ -77,34 +105,24 @@ __device__ __forceinline__ bool decode_slot(const PagedCache& C, int64_t slot, i
     raise_error(&g_paged_err, kErrBadPage);
     return false;
   }
-  page = slot / C.page_size;
+  page = slot < (int64_t(1) << 31) ? (int64_t)C.page_of((unsigned)slot) : slot / C.page_size;
   at = (int)(slot - page * C.page_size);
   return true;
 }
 
-__global__ void __launch_bounds__(256) kv_write_copy_kernel(const KvWriteArgs A) {
-  const unsigned row = blockIdx.x * 16u + threadIdx.x / 16u, c = threadIdx.x % 16u;
-  if (row >= A.rows) return;
-  const unsigned tok = row / A.hk, h = row - tok * A.hk;
-  const uint4 kx = __ldcs(reinterpret_cast<const uint4*>(A.k + tok * A.ks_tok + h * A.ks_head) + c);
-  const uint4 vx = __ldcs(reinterpret_cast<const uint4*>(A.v + tok * A.vs_tok + h * A.vs_head) + c);
-  int64_t page;
-  int at;
-  if (!decode_slot(A.C, load_slot(A, tok), page, at)) return;
-  const int64_t off = page * A.C.s_page + at * A.C.s_tok + h * A.C.s_head;
-  reinterpret_cast<uint4*>(A.C.k + off)[c] = kx;
-  reinterpret_cast<uint4*>(A.C.v + off)[c] = vx;
-}
+constexpr int kRowThreads = 256;
+constexpr int row_lanes(bool quantise) { return quantise ? 8 : 16; }                      // lanes of a row
+constexpr int block_rows(bool quantise) { return kRowThreads / row_lanes(quantise); }  // rows of a block at a time
 
-// One lane's 16 elements of a row: amax over the 8 lanes of the row, then codes and (first lane) the scale.
+// One lane's 16 elements of a row: amax over the row's 8 lanes, then the codes and (first lane) the scale.
 template <typename T>
-__device__ __forceinline__ void quantise_row(const uint4 (&x)[2], uint8_t* dst, float* scale, unsigned c, unsigned mask) {
+__device__ __forceinline__ void quantise_row(const uint4 (&x)[2], uint4* dst, float* scale, unsigned c, unsigned mask) {
   const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = absmax2(m, w[i]);
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(mask, m, o));
+  for (int o = 1; o < row_lanes(true); o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(mask, m, o));
   m = max(m & 0xFFFFu, m >> 16);
   float amax = DT<T>::lo(m);
   amax = amax < kAmaxFloor ? kAmaxFloor : amax;  // NaN stays NaN
@@ -112,29 +130,42 @@ __device__ __forceinline__ void quantise_row(const uint4 (&x)[2], uint8_t* dst, 
   uint32_t out[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    out[i] = f32x2_to_e4m3x2(DT<T>::lo(w[2 * i]) * inv, DT<T>::hi(w[2 * i]) * inv) |
-             f32x2_to_e4m3x2(DT<T>::lo(w[2 * i + 1]) * inv, DT<T>::hi(w[2 * i + 1]) * inv) << 16;
-  reinterpret_cast<uint4*>(dst)[c] = make_uint4(out[0], out[1], out[2], out[3]);
+    out[i] = f32x2_to_e4m3x2(mul2(DT<T>::lo(w[2 * i]), DT<T>::hi(w[2 * i]), inv)) |
+             f32x2_to_e4m3x2(mul2(DT<T>::lo(w[2 * i + 1]), DT<T>::hi(w[2 * i + 1]), inv)) << 16;
+  dst[c] = make_uint4(out[0], out[1], out[2], out[3]);
   if (c == 0) *scale = __fdiv_rn(amax, kE4m3Max);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) kv_write_e4m3_kernel(const KvWriteArgs A) {
-  const unsigned row = blockIdx.x * 32u + threadIdx.x / 8u, c = threadIdx.x % 8u;
+// T: type of the rows (a 16-bit cache gets a copy whatever it is).
+template <typename T, bool kE4m3>
+__global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvWriteArgs A) {
+  constexpr int kLanes = row_lanes(kE4m3), kPieces = 16 / kLanes;  // 16-byte pieces of a lane
+  const unsigned c = threadIdx.x % kLanes, row = blockIdx.x * block_rows(kE4m3) + threadIdx.x / kLanes;
   if (row >= A.rows) return;
-  const unsigned tok = row / A.hk, h = row - tok * A.hk;
-  const uint4* kp = reinterpret_cast<const uint4*>(A.k + tok * A.ks_tok + h * A.ks_head) + 2 * c;
-  const uint4* vp = reinterpret_cast<const uint4*>(A.v + tok * A.vs_tok + h * A.vs_head) + 2 * c;
-  const uint4 kx[2] = {__ldcs(kp), __ldcs(kp + 1)};
-  const uint4 vx[2] = {__ldcs(vp), __ldcs(vp + 1)};
+  const unsigned tok = A.token_of(row), h = row - tok * A.hk;
+  const int64_t slot = load_slot(A, tok);
+  const uint4* kp = reinterpret_cast<const uint4*>(A.k) + A.kp.at(0, tok, h) + c * kPieces;
+  const uint4* vp = reinterpret_cast<const uint4*>(A.v) + A.vp.at(0, tok, h) + c * kPieces;
+  uint4 kx[kPieces], vx[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) kx[i] = __ldcs(kp + i);
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) vx[i] = __ldcs(vp + i);
   int64_t page;
   int at;
-  if (!decode_slot(A.C, load_slot(A, tok), page, at)) return;  // the same for all 8 lanes of a row
-  const unsigned mask = 0xFFu << (threadIdx.x & 24u);
-  const int64_t off = page * A.C.s_page + at * A.C.s_tok + h * A.C.s_head;
-  const int64_t soff = page * A.C.ss_page + at * A.C.ss_tok + h * A.C.ss_head;
-  quantise_row<T>(kx, A.C.k + off, A.C.k_scale + soff, c, mask);
-  quantise_row<T>(vx, A.C.v + off, A.C.v_scale + soff, c, mask);
+  if (!decode_slot(A.C, slot, page, at)) return;  // the same for all lanes of a row
+  const uint64_t off = A.C.rows.at((unsigned)page, at, h);
+  uint4* ko = reinterpret_cast<uint4*>(A.C.k) + off;
+  uint4* vo = reinterpret_cast<uint4*>(A.C.v) + off;
+  if constexpr (kE4m3) {
+    const unsigned mask = 0xFFu << (threadIdx.x & 24u);
+    const uint64_t soff = A.C.scales.at((unsigned)page, at, h);
+    quantise_row<T>(kx, ko, A.C.k_scale + soff, c, mask);
+    quantise_row<T>(vx, vo, A.C.v_scale + soff, c, mask);
+  } else {
+    ko[c] = kx[0];
+    vo[c] = vx[0];
+  }
 }
 
 // ------------------------------------------------------------------ read
@@ -145,73 +176,82 @@ struct KvReadArgs {
   int max_pages;
   const int* seq_lens;
   int out_len, hk;
+  FastDiv group_of;  // item / hk
   uint8_t *k, *v;
-  int64_t ks_b, ks_tok, ks_head, vs_b, vs_tok, vs_head;  // bytes
+  Pitch kp, vp;      // outer: sequence
 };
 
-// Cached row (b, s, h) of the item `row` = s * hk + h; false where there is none to copy.
-__device__ __forceinline__ bool read_row(const KvReadArgs& A, unsigned row, int b, int& s, int& h, int64_t& page, int& at) {
-  s = row / (unsigned)A.hk;
-  h = row - s * A.hk;
-  const int len = __ldg(A.seq_lens + b);
-  const int64_t room = min((int64_t)A.max_pages * A.C.page_size, (int64_t)A.out_len);
-  if (len < 0 || len > room) {
-    raise_error(&g_paged_err, kErrBadLength);
-    return false;
-  }
-  if (s >= len) return false;
-  const int p = s / A.C.page_size;
-  at = s - p * A.C.page_size;
-  page = __ldg(A.page_table + b * A.table_stride + p);
-  if (page < 0 || page >= A.C.num_pages) {
-    raise_error(&g_paged_err, kErrBadPage);
-    return false;
-  }
-  return true;
-}
-
-__global__ void __launch_bounds__(256) kv_read_copy_kernel(const KvReadArgs A) {
-  const unsigned row = blockIdx.x * 16u + threadIdx.x / 16u, c = threadIdx.x % 16u;
-  const int b = blockIdx.y;
-  if (row >= (unsigned)A.out_len * (unsigned)A.hk) return;
-  int s, h, at;
-  int64_t page;
-  if (!read_row(A, row, b, s, h, page, at)) return;
-  const int64_t off = page * A.C.s_page + at * A.C.s_tok + h * A.C.s_head;
-  const uint4 kx = __ldg(reinterpret_cast<const uint4*>(A.C.k + off) + c);
-  const uint4 vx = __ldg(reinterpret_cast<const uint4*>(A.C.v + off) + c);
-  reinterpret_cast<uint4*>(A.k + b * A.ks_b + s * A.ks_tok + h * A.ks_head)[c] = kx;
-  reinterpret_cast<uint4*>(A.v + b * A.vs_b + s * A.vs_tok + h * A.vs_head)[c] = vx;
-}
-
 template <typename T>
-__device__ __forceinline__ void dequantise_row(uint4 x, float scale, uint4* dst) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t out[8];
+__device__ __forceinline__ uint4 dequantise8(uint2 x, float scale) {
+  const uint32_t p[4] = {e4m3x2_to_f16x2(x.x), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y), e4m3x2_to_f16x2(x.y >> 16)};
+  uint32_t out[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t p = e4m3x2_to_f16x2(i & 1 ? w[i / 2] >> 16 : w[i / 2]);
-    out[i] = DT<T>::pack(DT<__half>::lo(p) * scale, DT<__half>::hi(p) * scale);
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = mul2(DT<__half>::lo(p[i]), DT<__half>::hi(p[i]), scale);
+    out[i] = DT<T>::pack(f.x, f.y);
   }
-  dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
-  dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+  return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) kv_read_e4m3_kernel(const KvReadArgs A) {
-  const unsigned row = blockIdx.x * 32u + threadIdx.x / 8u, c = threadIdx.x % 8u;
-  const int b = blockIdx.y;
-  if (row >= (unsigned)A.out_len * (unsigned)A.hk) return;
-  int s, h, at;
-  int64_t page;
-  if (!read_row(A, row, b, s, h, page, at)) return;
-  const int64_t off = page * A.C.s_page + at * A.C.s_tok + h * A.C.s_head;
-  const int64_t soff = page * A.C.ss_page + at * A.C.ss_tok + h * A.C.ss_head;
-  const uint4 kx = __ldg(reinterpret_cast<const uint4*>(A.C.k + off) + c);
-  const uint4 vx = __ldg(reinterpret_cast<const uint4*>(A.C.v + off) + c);
-  const float ks = __ldg(A.C.k_scale + soff), vs = __ldg(A.C.v_scale + soff);
-  dequantise_row<T>(kx, ks, reinterpret_cast<uint4*>(A.k + b * A.ks_b + s * A.ks_tok + h * A.ks_head) + 2 * c);
-  dequantise_row<T>(vx, vs, reinterpret_cast<uint4*>(A.v + b * A.vs_b + s * A.vs_tok + h * A.vs_head) + 2 * c);
+// T: type of the rows (a 16-bit cache is copied whatever it is).  16 lanes take kGroup tokens of one head, all on one page
+// (kGroup divides page_size); y: sequence.
+template <typename T, bool kE4m3, int kGroup>
+__global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvReadArgs A) {
+  constexpr int kLanes = row_lanes(false);
+  const unsigned c = threadIdx.x % kLanes, item = blockIdx.x * block_rows(false) + threadIdx.x / kLanes;
+  const int b = blockIdx.y, len = __ldg(A.seq_lens + b);
+  if (len < 0 || len > min((int64_t)A.max_pages * A.C.page_size, (int64_t)A.out_len)) {
+    raise_error(&g_paged_err, kErrBadLength);
+    return;
+  }
+  const int group = A.group_of(item), h = item - group * A.hk, s = group * kGroup, n = len - s;
+  if (n <= 0) return;
+  const int p = A.C.page_of(s), at = s - p * A.C.page_size;
+  const int page = __ldg(A.page_table + b * A.table_stride + p);
+  if ((unsigned)page >= (unsigned)A.C.num_pages) {
+    raise_error(&g_paged_err, kErrBadPage);
+    return;
+  }
+  uint4* ko = reinterpret_cast<uint4*>(A.k) + A.kp.at(b, s, h) + c;
+  uint4* vo = reinterpret_cast<uint4*>(A.v) + A.vp.at(b, s, h) + c;
+  const uint64_t off = A.C.rows.at(page, at, h);
+  if constexpr (kE4m3) {
+    const uint2* kc = reinterpret_cast<const uint2*>(reinterpret_cast<const uint4*>(A.C.k) + off) + c;
+    const uint2* vc = reinterpret_cast<const uint2*>(reinterpret_cast<const uint4*>(A.C.v) + off) + c;
+    const uint64_t soff = A.C.scales.at(page, at, h);
+    uint2 kx[kGroup], vx[kGroup];
+    float ks[kGroup], vs[kGroup];
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j)
+      if (j < n) {
+        kx[j] = __ldg(kc + (uint64_t)j * 2 * A.C.rows.tok);
+        vx[j] = __ldg(vc + (uint64_t)j * 2 * A.C.rows.tok);
+        ks[j] = __ldg(A.C.k_scale + soff + (uint64_t)j * A.C.scales.tok);
+        vs[j] = __ldg(A.C.v_scale + soff + (uint64_t)j * A.C.scales.tok);
+      }
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j)
+      if (j < n) {
+        ko[(uint64_t)j * A.kp.tok] = dequantise8<T>(kx[j], ks[j]);
+        vo[(uint64_t)j * A.vp.tok] = dequantise8<T>(vx[j], vs[j]);
+      }
+  } else {
+    const uint4* kc = reinterpret_cast<const uint4*>(A.C.k) + off + c;
+    const uint4* vc = reinterpret_cast<const uint4*>(A.C.v) + off + c;
+    uint4 kx[kGroup], vx[kGroup];
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j)
+      if (j < n) {
+        kx[j] = __ldg(kc + (uint64_t)j * A.C.rows.tok);
+        vx[j] = __ldg(vc + (uint64_t)j * A.C.rows.tok);
+      }
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j)
+      if (j < n) {
+        ko[(uint64_t)j * A.kp.tok] = kx[j];
+        vo[(uint64_t)j * A.vp.tok] = vx[j];
+      }
+  }
 }
 
 __global__ void paged_clear_err_kernel(uint32_t bits) { atomicAnd(&g_paged_err, ~bits); }

@@ -3,6 +3,20 @@
 namespace fpb {
 namespace {
 
+FastDiv make_div(int d) {
+  int log2 = 0;
+  while ((int64_t(1) << log2) < d) ++log2;
+  return {(unsigned)((uint64_t(1) << (31 + log2)) / d + 1), 31 + log2};
+}
+
+// Strides in units of `unit`; each must be below 2^32 units.
+int make_pitch(Pitch* p, int64_t outer, int64_t tok, int64_t head, int unit, const char* what) {
+  for (const int64_t s : {outer, tok, head})
+    FPB_CHECK_ARG(s / unit < (int64_t(1) << 32), "%s stride of %lld %s is too large", what, (long long)s, unit > 1 ? "bytes" : "elements");
+  *p = {(unsigned)(outer / unit), (unsigned)(tok / unit), (unsigned)(head / unit)};
+  return FPB_OK;
+}
+
 // The cache arguments shared by the three entry points.  out: C with byte strides.
 int make_cache(PagedCache* C, const void* k_cache, const void* v_cache, int cache_dtype, int dtype, int num_pages,
                int page_size, int hk, int head_dim, const int64_t* cs, const float* k_scale, const float* v_scale,
@@ -20,29 +34,24 @@ int make_cache(PagedCache* C, const void* k_cache, const void* v_cache, int cach
   for (int i = 0; i < 3; ++i) {
     FPB_CHECK_ARG(cs[i] >= 0 && cs[i] * elt % 16 == 0, "cache stride[%d]=%lld must be a non-negative multiple of 16 bytes", i,
                   (long long)cs[i]);
-    FPB_CHECK_ARG(cs[i] < (int64_t(1) << 40), "cache stride[%d] too large", i);
   }
   C->k = static_cast<uint8_t*>(const_cast<void*>(k_cache));
   C->v = static_cast<uint8_t*>(const_cast<void*>(v_cache));
-  C->s_page = cs[0] * elt;
-  C->s_tok = cs[1] * elt;
-  C->s_head = cs[2] * elt;
+  FPB_TRY(make_pitch(&C->rows, cs[0] * elt, cs[1] * elt, cs[2] * elt, 16, "cache"));
   C->num_pages = num_pages;
   C->page_size = page_size;
+  C->page_of = make_div(page_size);
   C->k_scale = C->v_scale = nullptr;
-  C->ss_page = C->ss_tok = C->ss_head = 0;
+  C->scales = Pitch{0, 0, 0};
   if (cache_dtype == FPB_E4M3) {
     FPB_CHECK_ARG(k_scale != nullptr && v_scale != nullptr, "an e4m3 cache needs k_scale and v_scale");
     FPB_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) & 3) == 0,
                   "k_scale and v_scale must be aligned float pointers");
     FPB_CHECK_ARG(ss != nullptr, "scale strides are NULL");
-    for (int i = 0; i < 3; ++i)
-      FPB_CHECK_ARG(ss[i] >= 0 && ss[i] < (int64_t(1) << 40), "scale stride[%d]=%lld is out of range", i, (long long)ss[i]);
+    for (int i = 0; i < 3; ++i) FPB_CHECK_ARG(ss[i] >= 0, "scale stride[%d]=%lld is negative", i, (long long)ss[i]);
+    FPB_TRY(make_pitch(&C->scales, ss[0], ss[1], ss[2], 1, "scale"));
     C->k_scale = const_cast<float*>(k_scale);
     C->v_scale = const_cast<float*>(v_scale);
-    C->ss_page = ss[0];
-    C->ss_tok = ss[1];
-    C->ss_head = ss[2];
   } else {
     FPB_CHECK_ARG(k_scale == nullptr && v_scale == nullptr, "a 16-bit cache takes no scales");
   }
@@ -57,6 +66,21 @@ int check_table(const int32_t* table, int64_t stride, int max_pages, int page_si
   FPB_CHECK_ARG(seq_lens != nullptr && (reinterpret_cast<uintptr_t>(seq_lens) & 3) == 0,
                 "seq_lens must be an aligned int32 pointer");
   FPB_CHECK_ARG(stride >= 0 && stride < (int64_t(1) << 40), "page_table stride %lld is out of range", (long long)stride);
+  return FPB_OK;
+}
+
+// Launches a read kernel with one token of a head for 16 lanes, or with kReadGroup where page_size allows it and every SM
+// still gets the 8 blocks it holds.
+constexpr int kReadGroup = 4;
+template <typename T, bool kE4m3>
+int launch_read(const KvReadArgs& A, int batch, cudaStream_t stream) {
+  constexpr int kBlock = block_rows(false);
+  const bool grouped = A.C.page_size % kReadGroup == 0 && (int64_t)A.out_len * A.hk * batch >= (int64_t)kReadGroup * kBlock * 148 * 8;
+  const unsigned per = grouped ? kReadGroup : 1, items = ((unsigned)A.out_len + per - 1) / per * (unsigned)A.hk;
+  const dim3 grid((items + kBlock - 1) / kBlock, batch);
+  if (grouped) kv_read_kernel<T, kE4m3, kReadGroup><<<grid, kRowThreads, 0, stream>>>(A);
+  else kv_read_kernel<T, kE4m3, 1><<<grid, kRowThreads, 0, stream>>>(A);
+  FPB_CUDA(cudaGetLastError());
   return FPB_OK;
 }
 
@@ -94,7 +118,7 @@ DecodeShape decode_shape(int batch, int hq, int hk, int cache_dtype, int max_pag
   s.by_item = s.items <= s.pieces;
   // heads share a CTA of the join where an item has few pieces, and have one each where it has many
   const int64_t each = s.pieces / s.items;
-  s.join_heads = each >= 16 ? 1 : each >= 4 ? 2 : std::min(s.nh, kJoinThreads / 32);
+  s.join_heads = each >= 16 ? 1 : each >= 2 ? std::min(s.nh, 2) : std::min(s.nh, kJoinThreads / 32);
   return s;
 }
 int decode_descs(const DecodeShape& s) { return s.by_item ? (int)s.items : s.pieces; }
@@ -152,7 +176,7 @@ int fpb_kv_cache_write(const void* k, const void* v, int dtype, int tokens, int 
   FPB_TRY(make_cache(&A.C, k_cache, v_cache, cache_dtype, dtype, num_pages, page_size, hk, head_dim, cache_strides, k_scale,
                      v_scale, scale_strides));
   FPB_CHECK_ARG(tokens >= 0, "tokens (%d) must be >= 0", tokens);
-  FPB_CHECK_ARG((int64_t)tokens * hk < (int64_t(1) << 31), "tokens * num_kv_heads must be below 2^31");
+  FPB_CHECK_ARG((int64_t)tokens * hk < (int64_t(1) << 31) - 32, "tokens * num_kv_heads must be below 2^31");
   FPB_CHECK_ARG(slot_bytes == 4 || slot_bytes == 8, "slot_bytes must be 4 or 8 (got %d)", slot_bytes);
   if (tokens == 0) return FPB_OK;
   FPB_TRY(check_ptr(k, "k"));
@@ -162,18 +186,18 @@ int fpb_kv_cache_write(const void* k, const void* v, int dtype, int tokens, int 
   FPB_CHECK_ARG(slots != nullptr && reinterpret_cast<uintptr_t>(slots) % slot_bytes == 0, "slots must be an aligned pointer");
   A.k = static_cast<const uint8_t*>(k);
   A.v = static_cast<const uint8_t*>(v);
-  A.ks_tok = 2 * k_strides[0];
-  A.ks_head = 2 * k_strides[1];
-  A.vs_tok = 2 * v_strides[0];
-  A.vs_head = 2 * v_strides[1];
+  FPB_TRY(make_pitch(&A.kp, 0, 2 * k_strides[0], 2 * k_strides[1], 16, "k"));
+  FPB_TRY(make_pitch(&A.vp, 0, 2 * v_strides[0], 2 * v_strides[1], 16, "v"));
+  A.token_of = make_div(hk);
   A.slots = slots;
   A.slots64 = slot_bytes == 8;
   A.rows = (unsigned)tokens * (unsigned)hk;
   A.hk = hk;
   auto st = static_cast<cudaStream_t>(stream);
-  if (cache_dtype != FPB_E4M3) kv_write_copy_kernel<<<(A.rows + 15) / 16, 256, 0, st>>>(A);
-  else if (dtype == FPB_BF16) kv_write_e4m3_kernel<__nv_bfloat16><<<(A.rows + 31) / 32, 256, 0, st>>>(A);
-  else kv_write_e4m3_kernel<__half><<<(A.rows + 31) / 32, 256, 0, st>>>(A);
+  const unsigned per = block_rows(cache_dtype == FPB_E4M3), blocks = (A.rows + per - 1) / per;
+  if (cache_dtype != FPB_E4M3) kv_write_kernel<__half, false><<<blocks, kRowThreads, 0, st>>>(A);
+  else if (dtype == FPB_BF16) kv_write_kernel<__nv_bfloat16, true><<<blocks, kRowThreads, 0, st>>>(A);
+  else kv_write_kernel<__half, true><<<blocks, kRowThreads, 0, st>>>(A);
   FPB_CUDA(cudaGetLastError());
   return FPB_OK;
 }
@@ -188,7 +212,7 @@ int fpb_kv_cache_read(const void* k_cache, const void* v_cache, int cache_dtype,
                      v_scale, scale_strides));
   FPB_TRY(check_table(page_table, table_stride, max_pages, page_size, seq_lens, batch));
   FPB_CHECK_ARG(batch <= 65535, "batch (%d) must be at most 65535", batch);
-  FPB_CHECK_ARG(out_len >= 1 && (int64_t)out_len * hk < (int64_t(1) << 31), "out_len (%d) must be >= 1 and out_len * num_kv_heads below 2^31",
+  FPB_CHECK_ARG(out_len >= 1 && ((int64_t)out_len + 3) * hk < (int64_t(1) << 31) - 16, "out_len (%d) must be >= 1 and out_len * num_kv_heads below 2^31",
                 out_len);
   FPB_TRY(check_ptr(k, "k"));
   FPB_TRY(check_ptr(v, "v"));
@@ -202,19 +226,12 @@ int fpb_kv_cache_read(const void* k_cache, const void* v_cache, int cache_dtype,
   A.hk = hk;
   A.k = static_cast<uint8_t*>(k);
   A.v = static_cast<uint8_t*>(v);
-  A.ks_b = 2 * k_strides[0];
-  A.ks_tok = 2 * k_strides[1];
-  A.ks_head = 2 * k_strides[2];
-  A.vs_b = 2 * v_strides[0];
-  A.vs_tok = 2 * v_strides[1];
-  A.vs_head = 2 * v_strides[2];
-  const unsigned rows = (unsigned)out_len * (unsigned)hk;
+  FPB_TRY(make_pitch(&A.kp, 2 * k_strides[0], 2 * k_strides[1], 2 * k_strides[2], 16, "k"));
+  FPB_TRY(make_pitch(&A.vp, 2 * v_strides[0], 2 * v_strides[1], 2 * v_strides[2], 16, "v"));
+  A.group_of = make_div(hk);
   auto st = static_cast<cudaStream_t>(stream);
-  if (cache_dtype != FPB_E4M3) kv_read_copy_kernel<<<dim3((rows + 15) / 16, batch), 256, 0, st>>>(A);
-  else if (dtype == FPB_BF16) kv_read_e4m3_kernel<__nv_bfloat16><<<dim3((rows + 31) / 32, batch), 256, 0, st>>>(A);
-  else kv_read_e4m3_kernel<__half><<<dim3((rows + 31) / 32, batch), 256, 0, st>>>(A);
-  FPB_CUDA(cudaGetLastError());
-  return FPB_OK;
+  if (cache_dtype != FPB_E4M3) return launch_read<__half, false>(A, batch, st);
+  return dtype == FPB_BF16 ? launch_read<__nv_bfloat16, true>(A, batch, st) : launch_read<__half, true>(A, batch, st);
 }
 
 size_t fpb_paged_decode_workspace_bytes(int batch, int hq, int hk, int cache_dtype, int max_pages, int page_size) {
@@ -275,11 +292,6 @@ int fpb_paged_decode(const void* q, int dtype, int batch, int hq, int hk, int he
   A.by_item = s.by_item;
   A.join_heads = s.join_heads;
   A.c = (float)(sm_scale * 1.4426950408889634);
-  int log2_page = 0;
-  while ((int64_t(1) << log2_page) < page_size) ++log2_page;
-  // exact for tokens below 2^31: the multiplier exceeds 2^shift / page_size by less than one
-  A.page_shift = 31 + log2_page;
-  A.page_mul = (unsigned)((uint64_t(1) << A.page_shift) / page_size + 1);
   A.page16 = page_size % 16 == 0;
   auto st = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == FPB_BF16, e4m3 = cache_dtype == FPB_E4M3, wide = s.nh > 8;

@@ -107,7 +107,8 @@ def test_decode_workspace_is_bounded():
     n = fp.paged_decode_workspace_bytes
     assert n(1, 32, 8, BF16, 8, 16) == n(256, 32, 8, BF16, 64, 16) == 0  # short sequences: one cluster an item
     mid, large = n(1, 1, 1, BF16, 129, 64), n(256, 32, 8, BF16, 8192, 128)
-    assert 0 < mid < large == n(1, 32, 8, BF16, 8192, 128) < 4 << 20  # by the GPU's blocks, not by batch or length
+    # by the GPU's blocks and heads, not by batch or length
+    assert 0 < mid < large < 4 << 20 and abs(large - n(1, 32, 8, BF16, 8192, 128)) < 16384 and n(4096, 32, 8, BF16, 8192, 128) == large
     assert n(1, 128, 8, BF16, 8192, 128) > large  # 16 heads an item
     assert n(0, 32, 8, BF16, 8, 16) == n(1, 7, 2, BF16, 8, 16) == 0
 
