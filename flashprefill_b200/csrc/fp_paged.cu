@@ -138,7 +138,7 @@ __device__ __forceinline__ void quantise_row(const uint4 (&x)[2], uint4* dst, fl
 
 // T: type of the rows (a 16-bit cache gets a copy whatever it is).
 template <typename T, bool kE4m3>
-__global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvWriteArgs A) {
+__global__ void __launch_bounds__(kRowThreads, kE4m3 ? 6 : 8) kv_write_kernel(const KvWriteArgs A) {
   constexpr int kLanes = row_lanes(kE4m3), kPieces = 16 / kLanes;  // 16-byte pieces of a lane
   const unsigned c = threadIdx.x % kLanes, row = blockIdx.x * block_rows(kE4m3) + threadIdx.x / kLanes;
   if (row >= A.rows) return;
@@ -148,9 +148,9 @@ __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvWriteArgs
   const uint4* vp = reinterpret_cast<const uint4*>(A.v) + A.vp.at(0, tok, h) + c * kPieces;
   uint4 kx[kPieces], vx[kPieces];
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) kx[i] = __ldcs(kp + i);
+  for (int i = 0; i < kPieces; ++i) kx[i] = __ldg(kp + i);
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) vx[i] = __ldcs(vp + i);
+  for (int i = 0; i < kPieces; ++i) vx[i] = __ldg(vp + i);
   int64_t page;
   int at;
   if (!decode_slot(A.C, slot, page, at)) return;  // the same for all lanes of a row
