@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
   __shared__ float2 s_ml[kDecWarps][8 * NT];
   static_assert(8 * NT * 132 * 4 <= kDecRingBytes, "a warp's sums fit its ring");
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  await_stream();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int HH = A.hk * A.ngroups, v = blockIdx.x;
 
@@ -663,6 +663,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
   __shared__ float2 s_ml[kDecWarps][8 * NT];
   __shared__ float s_x[8 * NT][kHeadDim];  // this CTA's sums, read by the others of the cluster
   __shared__ float2 s_cta[8 * NT];
+  await_stream();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int item = blockIdx.x / cluster, rank = blockIdx.x - item * cluster;
   const int HH = A.hk * A.ngroups, b = item / HH, hh = item - b * HH;
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_decode_join_kernel(const D
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int parts = kWarps / A.join_heads;  // join_heads <= kWarps
   const int part = warp / A.join_heads, i = blockIdx.y * A.join_heads + warp % A.join_heads;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  await_stream();
   const int4 d = A.desc[blockIdx.x];
   const int n = d.w;
   if (n == 0) return;

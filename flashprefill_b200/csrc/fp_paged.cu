@@ -62,6 +62,12 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)two));
   return r;
 }
+// The kernels of the paged cache are short and follow one another (write, decode, join, the next layer's write ...), so each
+// is launched with programmatic stream serialisation, which prepares its launch while its predecessor still runs, and waits here, before it touches
+// memory, until all that came before it on the stream is complete and visible (1 x 500 tokens decode: 6.2 us a call
+// without, 4.6 with).
+__device__ __forceinline__ void await_stream() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // (a0, a1) * b, two products in one instruction
 __device__ __forceinline__ float2 mul2(float a0, float a1, float b) {
   float2 d;
@@ -140,6 +146,7 @@ __device__ __forceinline__ void quantise_row(const uint4 (&x)[2], uint4* dst, fl
 template <typename T, bool kE4m3>
 __global__ void __launch_bounds__(kRowThreads, kE4m3 ? 6 : 8) kv_write_kernel(const KvWriteArgs A) {
   constexpr int kLanes = row_lanes(kE4m3), kPieces = 16 / kLanes;  // 16-byte pieces of a lane
+  await_stream();
   const unsigned c = threadIdx.x % kLanes, row = blockIdx.x * block_rows(kE4m3) + threadIdx.x / kLanes;
   if (row >= A.rows) return;
   const unsigned tok = A.token_of(row), h = row - tok * A.hk;
@@ -198,6 +205,7 @@ __device__ __forceinline__ uint4 dequantise8(uint2 x, float scale) {
 template <typename T, bool kE4m3, int kGroup>
 __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvReadArgs A) {
   constexpr int kLanes = row_lanes(false);
+  await_stream();
   const unsigned c = threadIdx.x % kLanes, item = blockIdx.x * block_rows(false) + threadIdx.x / kLanes;
   const int b = blockIdx.y, len = __ldg(A.seq_lens + b);
   if (len < 0 || len > min((int64_t)A.max_pages * A.C.page_size, (int64_t)A.out_len)) {

@@ -69,6 +69,26 @@ int check_table(const int32_t* table, int64_t stride, int max_pages, int page_si
   return FPB_OK;
 }
 
+// Launches a kernel that begins with await_stream(), in clusters of `cluster` CTAs.
+template <typename... P, typename... V>
+int launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, const V&... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attrs[2] = {};
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  FPB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return FPB_OK;
+}
+
 // Launches a read kernel with one token of a head for 16 lanes, or with kReadGroup where page_size allows it and every SM
 // still gets the 8 blocks it holds.
 constexpr int kReadGroup = 4;
@@ -78,10 +98,7 @@ int launch_read(const KvReadArgs& A, int batch, cudaStream_t stream) {
   const bool grouped = A.C.page_size % kReadGroup == 0 && (int64_t)A.out_len * A.hk * batch >= (int64_t)kReadGroup * kBlock * 148 * 8;
   const unsigned per = grouped ? kReadGroup : 1, items = ((unsigned)A.out_len + per - 1) / per * (unsigned)A.hk;
   const dim3 grid((items + kBlock - 1) / kBlock, batch);
-  if (grouped) kv_read_kernel<T, kE4m3, kReadGroup><<<grid, kRowThreads, 0, stream>>>(A);
-  else kv_read_kernel<T, kE4m3, 1><<<grid, kRowThreads, 0, stream>>>(A);
-  FPB_CUDA(cudaGetLastError());
-  return FPB_OK;
+  return launch(grouped ? kv_read_kernel<T, kE4m3, kReadGroup> : kv_read_kernel<T, kE4m3, 1>, grid, kRowThreads, 0, 1, stream, A);
 }
 
 // How the query heads of a KV head become items: equal groups of at most 16.
@@ -132,35 +149,16 @@ int64_t decode_ws_total(const DecodeShape& s) {
 
 template <typename T, bool kE4m3, int NT>
 int launch_decode(const DecodeArgs& A, const DecodeShape& s, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.blockDim = dim3(kDecThreads);
-  cfg.dynamicSmemBytes = kDecSmemBytes;
   if (s.cluster) {
     auto kernel = paged_decode_short_kernel<T, kE4m3, NT>;
     FPB_TRY(set_smem(kernel, kDecSmemBytes));
-    cfg.gridDim = dim3((unsigned)(s.items * s.cluster));
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = s.cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.numAttrs = s.cluster > 1;
-    FPB_CUDA(cudaLaunchKernelEx(&cfg, kernel, A, s.cluster));
-    return FPB_OK;
+    return launch(kernel, dim3((unsigned)(s.items * s.cluster)), kDecThreads, kDecSmemBytes, s.cluster, stream, A, s.cluster);
   }
   auto kernel = paged_decode_kernel<T, kE4m3, NT>;
   FPB_TRY(set_smem(kernel, kDecSmemBytes));
-  cfg.gridDim = dim3(s.pieces);
-  FPB_CUDA(cudaLaunchKernelEx(&cfg, kernel, A));
-  cfg.gridDim = dim3(decode_descs(s), (s.nh + s.join_heads - 1) / s.join_heads);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.dynamicSmemBytes = 0;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.numAttrs = 1;
-  FPB_CUDA(cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<T>, A));
-  return FPB_OK;
+  FPB_TRY(launch(kernel, dim3(s.pieces), kDecThreads, kDecSmemBytes, 1, stream, A));
+  return launch(paged_decode_join_kernel<T>, dim3(decode_descs(s), (s.nh + s.join_heads - 1) / s.join_heads), kJoinThreads, 0, 1,
+                stream, A);
 }
 
 }  // namespace
@@ -195,11 +193,10 @@ int fpb_kv_cache_write(const void* k, const void* v, int dtype, int tokens, int 
   A.hk = hk;
   auto st = static_cast<cudaStream_t>(stream);
   const unsigned per = block_rows(cache_dtype == FPB_E4M3), blocks = (A.rows + per - 1) / per;
-  if (cache_dtype != FPB_E4M3) kv_write_kernel<__half, false><<<blocks, kRowThreads, 0, st>>>(A);
-  else if (dtype == FPB_BF16) kv_write_kernel<__nv_bfloat16, true><<<blocks, kRowThreads, 0, st>>>(A);
-  else kv_write_kernel<__half, true><<<blocks, kRowThreads, 0, st>>>(A);
-  FPB_CUDA(cudaGetLastError());
-  return FPB_OK;
+  return launch(cache_dtype != FPB_E4M3 ? kv_write_kernel<__half, false>
+                : dtype == FPB_BF16     ? kv_write_kernel<__nv_bfloat16, true>
+                                        : kv_write_kernel<__half, true>,
+                dim3(blocks), kRowThreads, 0, 1, st, A);
 }
 
 int fpb_kv_cache_read(const void* k_cache, const void* v_cache, int cache_dtype, int num_pages, int page_size, int hk,
