@@ -8,7 +8,7 @@
 // bound by HBM; the arithmetic only has to stay out of the way.
 //
 // An item is (sequence, KV head, group of query heads: all G up to 16, equal groups of at most 16 above that), its tokens are cut
-// into units of kDecWarps * TT.  Lengths are read on the device (no host copy; a captured graph serves any lengths).
+// into units of TT tokens for each warp of a CTA.  Lengths are read on the device (no host copy; a captured graph serves any lengths).
 //
 // Long sequences (paged_decode_kernel).  All items' units form one line, with one empty unit at the head of each item for
 // what starting an item costs, and each of the CTAs that the GPU holds takes an equal piece of it, so ragged batches and
@@ -30,10 +30,11 @@
 // tcgen05's least tile would be mostly padding, and the operands need no staging beyond the ring.
 //   * Scores, maxima, sums and outputs stay in fp32 registers.  The running maximum is reduced over the warp, and sums are
 //     rescaled, only in tiles where some score exceeds it.
-//   * bf16 V: P is split into two bf16 parts (the value and its remainder) and multiplied twice: one bf16 P would leave
-//     errors as large as the output's own rounding.
-//   * fp16 V: P is scaled by 2^15 (as the row sum is, so it cancels), which keeps weights down to 2^-29 of the largest in
-//     fp16's normal range.
+//   * P is split into two 16-bit parts (the value and its remainder) and multiplied twice: one part alone would leave errors
+//     as large as the output's own rounding.  Only for an e4m3 cache with bf16 output is one part enough: fp16 products, an
+//     eighth of the output's rounding.
+//   * fp16 products: P is scaled by 2^15 (as the row sum is, so it cancels), which keeps weights down to 2^-29 of the
+//     largest in fp16's normal range.
 //   * e4m3: codes widen to fp16 exactly; q is scaled by a power of two to fit fp16; the token's K scale multiplies its
 //     score and its V scale its weight, relative to the largest V scale so far (a running reference like the maximum), so
 //     weights stay at most 2^15.
@@ -43,15 +44,15 @@
 
 namespace fpb {
 
-constexpr int kDecWarps = 4;
 constexpr int kDecStages = 2;
-constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kDecTileBytes = 4096;  // one warp's tile of K or of V
 constexpr int kDecRingBytes = kDecStages * 2 * kDecTileBytes;
-constexpr int kDecSmemBytes = kDecWarps * kDecRingBytes;
-constexpr int dec_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }  // registers: 168 or 255 a thread
+// CTAs of narrow (4 warps) and wide form (as many as the registers hold: one CTA an SM), by 8s of heads of an item.
+constexpr int kNarrow = 4;
+constexpr int wide_warps(int nt) { return nt == 1 ? 12 : 8; }
+constexpr int dec_ctas_per_sm(int nt, int warps) { return wide_warps(nt) / warps; }
+constexpr int dec_smem_bytes(int warps) { return warps * kDecRingBytes; }
 constexpr int kDecMaxCluster = 8;
-static_assert(kDecThreads == kHeadDim, "one thread for each channel in the merges");
 constexpr int kJoinThreads = 256;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -140,8 +141,8 @@ struct DecodeWarp {
   static constexpr int kRowBytes = kDecTileBytes / TT;
   static constexpr int kChunks = kRowBytes / 16;  // 16-byte pieces of a row
   static constexpr uint32_t kFull = TT == 32 ? 0xFFFFFFFFu : 0xFFFFu;
-  static constexpr bool kSplitP = DT<MT>::is_bf16;
-  static constexpr float kShift = kSplitP ? 0.f : 15.f;  // log2 of the factor of P and l
+  static constexpr bool kSplitP = !(kE4m3 && DT<T>::is_bf16);    // P as two parts
+  static constexpr float kShift = DT<MT>::is_bf16 ? 0.f : 15.f;  // log2 of the factor of P and l
 
   uint32_t ring;  // shared address of this warp's ring
   int lane;
@@ -449,7 +450,10 @@ struct DecodeWarp {
           const uint32_t a0 = e4m3x2_to_f16x2(x), a1 = e4m3x2_to_f16x2(x >> 16);
           const uint32_t a2 = e4m3x2_to_f16x2(y), a3 = e4m3x2_to_f16x2(y >> 16);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<MT>(o[n][i], a0, a1, a2, a3, pb[n][k][0], pb[n][k][1]);
+          for (int n = 0; n < NT; ++n) {
+            mma16816<MT>(o[n][i], a0, a1, a2, a3, pb[n][k][0], pb[n][k][1]);
+            if constexpr (kSplitP) mma16816<MT>(o[n][i], a0, a1, a2, a3, pl[n][k][0], pl[n][k][1]);
+          }
         }
       }
     }
@@ -526,27 +530,27 @@ struct DecodeWarp {
   }
 };
 
-// Joins the warps' sums of head i at channel tid: {sum of weights times v, sum of weights, maximum}.
-template <int NT>
-__device__ __forceinline__ void merge_warps(const uint8_t* smem, const float2 (&s_ml)[kDecWarps][8 * NT], int i, int tid,
-                                            float& x, float& l, float& mx) {
+// Joins the warps' sums of head i at channel d: {sum of weights times v, sum of weights, maximum}.
+template <int kWarps, int NT>
+__device__ __forceinline__ void merge_warps(const uint8_t* smem, const float2 (&s_ml)[kWarps][8 * NT], int i, int d, float& x,
+                                            float& l, float& mx) {
   mx = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < kDecWarps; ++k) mx = fmaxf(mx, s_ml[k][i].x);
+  for (int k = 0; k < kWarps; ++k) mx = fmaxf(mx, s_ml[k][i].x);
   const float ref = finite_or_zero(mx);
   l = x = 0.f;
 #pragma unroll
-  for (int k = 0; k < kDecWarps; ++k) {
+  for (int k = 0; k < kWarps; ++k) {
     const float f = ex2_approx(s_ml[k][i].x - ref);
     l += f * s_ml[k][i].y;
-    x += f * reinterpret_cast<const float*>(smem + k * kDecRingBytes)[i * 132 + tid];
+    x += f * reinterpret_cast<const float*>(smem + k * kDecRingBytes)[i * 132 + d];
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void write_head(const DecodeArgs& A, int b, int head, int tid, float x, float l, float mx) {
-  reinterpret_cast<T*>(A.out + b * A.o_b + head * A.o_h)[tid] = DT<T>::from_f(l == 0.f ? 0.f : x / l);
-  if (A.lse && tid == 0) A.lse[(int64_t)b * A.hq + head] = l == 0.f ? -INFINITY : (mx + log2f(l)) * kLn2;
+__device__ __forceinline__ void write_head(const DecodeArgs& A, int b, int head, int d, float x, float l, float mx) {
+  reinterpret_cast<T*>(A.out + b * A.o_b + head * A.o_h)[d] = DT<T>::from_f(l == 0.f ? 0.f : x / l);
+  if (A.lse && d == 0) A.lse[(int64_t)b * A.hq + head] = l == 0.f ? -INFINITY : (mx + log2f(l)) * kLn2;
 }
 
 // Equal cuts of `total` units into `n` pieces: piece i starts at i * q + min(i, r).
@@ -557,16 +561,16 @@ struct Cut {
   __device__ __forceinline__ int piece(int t) const { return t < r * (q + 1) ? t / (q + 1) : r + (t - r * (q + 1)) / q; }
 };
 
-template <typename T, bool kE4m3, int NT>
-__global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode_kernel(const DecodeArgs A) {
+template <typename T, bool kE4m3, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, dec_ctas_per_sm(NT, kWarps)) paged_decode_kernel(const DecodeArgs A) {
   using W = DecodeWarp<T, kE4m3, NT>;
-  constexpr int kUnit = kDecWarps * W::TT;
+  constexpr int kUnit = kWarps * W::TT;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 s_ml[kDecWarps][8 * NT];
+  __shared__ float2 s_ml[kWarps][8 * NT];
   static_assert(8 * NT * 132 * 4 <= kDecRingBytes, "a warp's sums fit its ring");
 
   await_stream();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = tid % kHeadDim;
   const int HH = A.hk * A.ngroups, v = blockIdx.x;
 
   // ---- this CTA's piece, found by every warp for itself: prefix sums of the sequences' units.  The host has checked that
@@ -626,14 +630,14 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
 
     const bool whole = u == 0 && u_end == units;
     const int64_t slot = 2 * v + (u == 0 ? 1 : 0);
-    for (int i = 0; i < heads; ++i) {
+    for (int i = tid / kHeadDim; i < heads; i += kWarps * 32 / kHeadDim) {
       float x, l, mx;
-      merge_warps<NT>(smem, s_ml, i, tid, x, l, mx);
+      merge_warps<kWarps, NT>(smem, s_ml, i, d, x, l, mx);
       if (whole) {
-        write_head<T>(A, b, head0 + i, tid, x, l, mx);
+        write_head<T>(A, b, head0 + i, d, x, l, mx);
       } else {
-        A.part[(slot * A.nh + i) * kHeadDim + tid] = x;
-        if (tid == 0) A.ml[slot * A.nh + i] = make_float2(mx, l);
+        A.part[(slot * A.nh + i) * kHeadDim + d] = x;
+        if (d == 0) A.ml[slot * A.nh + i] = make_float2(mx, l);
       }
     }
     if (u == 0 && tid == 0 && (A.by_item || !whole)) {
@@ -654,17 +658,17 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
   }
 }
 
-// One item for each cluster of `cluster` CTAs (a power of two up to 8); CTA r takes the units r, r + cluster, ...
-template <typename T, bool kE4m3, int NT>
-__global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode_short_kernel(const DecodeArgs A, int cluster) {
+// One item for each cluster of `cluster` CTAs (up to 8); CTA r takes the units r, r + cluster, ...
+template <typename T, bool kE4m3, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, dec_ctas_per_sm(NT, kWarps)) paged_decode_short_kernel(const DecodeArgs A, int cluster) {
   using W = DecodeWarp<T, kE4m3, NT>;
-  constexpr int kUnit = kDecWarps * W::TT;
+  constexpr int kUnit = kWarps * W::TT;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 s_ml[kDecWarps][8 * NT];
+  __shared__ float2 s_ml[kWarps][8 * NT];
   __shared__ float s_x[8 * NT][kHeadDim];  // this CTA's sums, read by the others of the cluster
   __shared__ float2 s_cta[8 * NT];
   await_stream();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = tid % kHeadDim;
   const int item = blockIdx.x / cluster, rank = blockIdx.x - item * cluster;
   const int HH = A.hk * A.ngroups, b = item / HH, hh = item - b * HH;
   const int h = hh / A.ngroups, grp = hh - h * A.ngroups;
@@ -675,20 +679,20 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
   w.run(A, b, h, head0, heads, rank * kUnit + warp * W::TT, cluster * kUnit, seq_len_of(A, b));
   w.store(reinterpret_cast<float*>(smem + warp * kDecRingBytes), s_ml[warp]);
   __syncthreads();
-  for (int i = 0; i < heads; ++i) {
+  for (int i = tid / kHeadDim; i < heads; i += kWarps * 32 / kHeadDim) {
     float x, l, mx;
-    merge_warps<NT>(smem, s_ml, i, tid, x, l, mx);
+    merge_warps<kWarps, NT>(smem, s_ml, i, d, x, l, mx);
     if (cluster == 1) {
-      write_head<T>(A, b, head0 + i, tid, x, l, mx);
+      write_head<T>(A, b, head0 + i, d, x, l, mx);
     } else {
-      s_x[i][tid] = x;
-      if (tid == 0) s_cta[i] = make_float2(mx, l);
+      s_x[i][d] = x;
+      if (d == 0) s_cta[i] = make_float2(mx, l);
     }
   }
   if (cluster == 1) return;
   cluster_sync();
-  for (int i = rank; i < heads; i += cluster) {
-    const uint32_t ax = smem_u32(&s_x[i][tid]), am = smem_u32(&s_cta[i]);
+  for (int i = rank + cluster * (tid / kHeadDim); i < heads; i += cluster * (kWarps * 32 / kHeadDim)) {
+    const uint32_t ax = smem_u32(&s_x[i][d]), am = smem_u32(&s_cta[i]);
     float2 ml[kDecMaxCluster];
     float xs[kDecMaxCluster], mx = -INFINITY;
 #pragma unroll
@@ -710,7 +714,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(NT)) paged_decode
       l += f * ml[k].y;
       x += f * xs[k];
     }
-    write_head<T>(A, b, head0 + i, tid, x, l, mx);
+    write_head<T>(A, b, head0 + i, d, x, l, mx);
   }
   cluster_sync();  // no CTA leaves while others read its sums
 }

@@ -108,13 +108,20 @@ void head_groups(int G, int* ngroups, int* nh) {
   *ngroups = (G + *nh - 1) / *nh;
 }
 
-// How a call runs.  Short sequences: clusters of the least power of two of CTAs that fills the GPU's places (at most 8, and
-// no more than an item can have units), if that leaves at most kShortUnits units to a CTA; else pieces of the line of all
-// units.  Every size here is a bound from the table's width: lengths are known on the device only.
-constexpr int kShortUnits = 16;
+// How a call runs.  Every size here is a bound from the table's width: lengths are known on the device only.
+//
+// Short sequences: a cluster for each item, if no warp gets more than kShortTiles tiles that way: as many CTAs as the GPU holds
+// at once, 8 at most.  Few items of more than kNarrowTiles tiles a warp take wide CTAs, so that a warp's tiles, one after
+// another, are fewer (32/8 heads, bf16: 1 x 4096 tokens 12.7 us with 4 warps, 9.3 with 12; 2 x 1024, 2 tiles a warp, 6.9 and 7.9).
+// Else pieces of the line of all units: 8192 tokens of one such sequence take 20 us in clusters of narrow CTAs, 15 in
+// pieces, 13 in clusters of wide ones; 256 x up to 600 tokens of 8/2 heads 20 in clusters and 22 in pieces.  Few items, each of several
+// pieces, take wide CTAs, which leave a third as many partial sums (2 x 262144 tokens, 28/4 heads, e4m3: 92 and 90 us); many
+// ragged ones narrow CTAs, which wait for one another less (64 x up to 8192: 171 and 174).
+constexpr int kSms = 148;
+constexpr int kShortTiles = 12, kNarrowTiles = 3;
 struct DecodeShape {
   int G, ngroups, nh;
-  int cluster;           // 0: pieces
+  int warps, cluster;    // of a CTA; cluster 0: pieces
   int pieces;            // CTAs: the places of a 148-SM GPU
   int by_item, join_heads;
   int64_t items, units;  // all items; all units at most
@@ -123,15 +130,19 @@ DecodeShape decode_shape(int batch, int hq, int hk, int cache_dtype, int max_pag
   DecodeShape s{};
   s.G = hq / hk;
   head_groups(s.G, &s.ngroups, &s.nh);
-  const int unit = kDecWarps * (cache_dtype == FPB_E4M3 ? 32 : 16);
-  const int places = 148 * dec_ctas_per_sm(s.nh <= 8 ? 1 : 2);
-  const int64_t units = ((int64_t)max_pages * page_size + unit - 1) / unit;
+  const int nt = s.nh <= 8 ? 1 : 2, tile = cache_dtype == FPB_E4M3 ? 32 : 16;
+  const int64_t tiles = ((int64_t)max_pages * page_size + tile - 1) / tile;
   s.items = (int64_t)batch * hk * s.ngroups;
-  s.units = s.items * (units + 1);
-  int cluster = 1;
-  while (cluster < kDecMaxCluster && 2 * cluster <= units && s.items * cluster < places) cluster *= 2;
-  s.cluster = (units + cluster - 1) / cluster <= kShortUnits && s.items * cluster < (int64_t(1) << 31) ? cluster : 0;
-  s.pieces = (int)std::min<int64_t>(places, s.units);
+  s.warps = s.items <= kSms && tiles > kNarrowTiles * kNarrow * kDecMaxCluster ? wide_warps(nt) : kNarrow;
+  const int64_t units = (tiles + s.warps - 1) / s.warps, places = kSms * dec_ctas_per_sm(nt, s.warps);
+  s.cluster = 1;
+  while (s.cluster < kDecMaxCluster && 2 * s.cluster <= units && s.items * 2 * s.cluster <= places) s.cluster *= 2;
+  if (tiles > (int64_t)kShortTiles * s.warps * s.cluster || s.items * s.cluster >= (int64_t(1) << 31)) {
+    s.cluster = 0;
+    s.warps = 2 * s.items <= kSms ? wide_warps(nt) : kNarrow;
+  }
+  s.units = s.items * ((tiles + s.warps - 1) / s.warps + 1);
+  s.pieces = (int)std::min<int64_t>(kSms * dec_ctas_per_sm(nt, s.warps), s.units);
   s.by_item = s.items <= s.pieces;
   // heads share a CTA of the join where an item has few pieces, and have one each where it has many
   const int64_t each = s.pieces / s.items;
@@ -149,14 +160,16 @@ int64_t decode_ws_total(const DecodeShape& s) {
 
 template <typename T, bool kE4m3, int NT>
 int launch_decode(const DecodeArgs& A, const DecodeShape& s, cudaStream_t stream) {
+  const int smem = dec_smem_bytes(s.warps);
   if (s.cluster) {
-    auto kernel = paged_decode_short_kernel<T, kE4m3, NT>;
-    FPB_TRY(set_smem(kernel, kDecSmemBytes));
-    return launch(kernel, dim3((unsigned)(s.items * s.cluster)), kDecThreads, kDecSmemBytes, s.cluster, stream, A, s.cluster);
+    auto kernel = s.warps == kNarrow ? paged_decode_short_kernel<T, kE4m3, NT, kNarrow>
+                                     : paged_decode_short_kernel<T, kE4m3, NT, wide_warps(NT)>;
+    FPB_TRY(set_smem(kernel, smem));
+    return launch(kernel, dim3((unsigned)(s.items * s.cluster)), s.warps * 32, smem, s.cluster, stream, A, s.cluster);
   }
-  auto kernel = paged_decode_kernel<T, kE4m3, NT>;
-  FPB_TRY(set_smem(kernel, kDecSmemBytes));
-  FPB_TRY(launch(kernel, dim3(s.pieces), kDecThreads, kDecSmemBytes, 1, stream, A));
+  auto kernel = s.warps == kNarrow ? paged_decode_kernel<T, kE4m3, NT, kNarrow> : paged_decode_kernel<T, kE4m3, NT, wide_warps(NT)>;
+  FPB_TRY(set_smem(kernel, smem));
+  FPB_TRY(launch(kernel, dim3(s.pieces), s.warps * 32, smem, 1, stream, A));
   return launch(paged_decode_join_kernel<T>, dim3(decode_descs(s), (s.nh + s.join_heads - 1) / s.join_heads), kJoinThreads, 0, 1,
                 stream, A);
 }

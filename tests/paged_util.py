@@ -94,7 +94,8 @@ def decode_bounds(ref, lse, weight, size, n, dtype, cache_dtype, q, k, v, sm_sca
       score: 128 products summed in fp32 and a few factors, at most (128 + 6) 2^-24 of sum |q_d k_d|, and for an e4m3 cache
         q's own step as fp16 below 2^-14 of its largest element, 2^-24 of that element for each d;
       exp2: 2^-22 relative, and its argument's rounding 2^-23 |s| (s in log2 units, bounded by the size of the score);
-      weights: fp16 2^-11 (bf16: two parts, 2^-16), fp16 steps of 2^-25 against a largest weight of 2^15 times the row's V scale;
+      weights: two bf16 parts 2^-16, two fp16 parts 2^-21, one fp16 part (e4m3 to bf16) 2^-11, and fp16 steps of 2^-25 against
+        a largest weight of 2^15 times the row's V scale;
       sums over n tokens in fp32: n 2^-24;  output: one rounding to its type."""
     if n == 0:
         return torch.zeros_like(ref), torch.zeros_like(lse)
@@ -106,7 +107,7 @@ def decode_bounds(ref, lse, weight, size, n, dtype, cache_dtype, q, k, v, sm_sca
     sums = (n + 16) * 2.0 ** -24
     rel = 2 * ds + sums + 2.0 ** -21
     fp16 = dtype is torch.float16 or cache_dtype is E4M3
-    wstep = 2.0 ** -11 if fp16 else 2.0 ** -16
+    wstep = 2.0 ** -11 if dtype is torch.bfloat16 and fp16 else 2.0 ** -21 if fp16 else 2.0 ** -16
     top = v.abs().amax().item()
     out_tol = half_step(dtype) * ref.abs() + (rel[:, None] + wstep) * weight + (n * 2.0 ** -40 * top if fp16 else 0.0) + \
         2.0 ** -25 * (dtype is torch.float16)
