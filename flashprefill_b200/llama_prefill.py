@@ -15,6 +15,9 @@ Weights are random (normal, std 0.02, bf16) and seeded per matrix, so every rank
 slice of one and the same full model for any number of ranks.  The GEMMs run on cuBLAS through
 torch (plain library GEMMs); the attention runs the library's CUDA kernels; RMSNorm, RoPE and SiLU
 are torch element-wise ops.
+
+``prefill`` and ``decode`` answer: they keep each layer's keys and values in a paged cache (``new_cache``), so a prompt can come
+in chunks and its answer token by token.  Each rank's cache holds its own KV heads.
 """
 from __future__ import annotations
 
@@ -43,6 +46,30 @@ class LlamaConfig:
     attention_sink: int = 2
     window: int = 4
     last_n: int = 2
+
+
+@dataclass
+class LlamaCache:
+    """One rank's keys and values of a batch of sequences: a paged cache for each layer, all with one page table.  ``lens`` is
+    the host's copy of ``seq_lens`` (tokens cached so far)."""
+    layers: list                # KVCache of every layer
+    page_table: torch.Tensor    # int32 (batch, pages)
+    seq_lens: torch.Tensor      # int32 (batch,)
+    lens: list
+    rope: tuple                 # cos, sin of every position that fits
+
+    @property
+    def page_size(self) -> int:
+        return self.layers[0].k.shape[1]
+
+    @property
+    def max_len(self) -> int:
+        return self.page_table.shape[1] * self.page_size
+
+    def slots(self, seq: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
+        """Cache slots of positions ``pos`` of sequences ``seq`` (int64 tensors of one shape)."""
+        ps = self.page_size
+        return self.page_table[seq, pos // ps].long() * ps + pos % ps
 
 
 def _seeded_normal(shape, seed, std, device, dtype):
@@ -119,6 +146,34 @@ class TPLlamaPrefill:
             (self.all_reduce or torch.distributed.all_reduce)(x)
         return x
 
+    def _layer(self, L, x, cos, sin, attend):
+        """One layer on the hidden rows x; ``attend(q, k, v)`` on (rows, heads, D) returns the attention as (rows, hq * D)."""
+        cfg = self.cfg
+        S, D = x.shape[0], cfg.head_dim
+        nq, nk = self.hq_l * D, self.hk_l * D
+        h = rms_norm(x, L["attn_norm"], cfg.eps)
+        qkv = h @ L["wqkv"].t()
+        q = apply_rope(qkv[:, :nq].view(S, self.hq_l, D), cos, sin)
+        k = apply_rope(qkv[:, nq:nq + nk].view(S, self.hk_l, D), cos, sin)
+        v = qkv[:, nq + nk:].view(S, self.hk_l, D)
+        del qkv
+        attn = attend(q, k, v)
+        del q, k, v
+        o = attn @ L["wo"].t()
+        x = x + self._reduce(o)
+        del o
+        h = rms_norm(x, L["mlp_norm"], cfg.eps)
+        gu = h @ L["wgu"].t()
+        a = torch.nn.functional.silu(gu[:, :self.f_l]) * gu[:, self.f_l:]
+        del gu
+        y = a @ L["wd"].t()
+        del a
+        return x + self._reduce(y)
+
+    def _logits(self, x):
+        last = rms_norm(x, self.final_norm, self.cfg.eps)
+        return last.float() @ self.lm_head.float().t()
+
     @torch.no_grad()
     def forward(self, tokens: torch.Tensor, events=None) -> torch.Tensor:
         """Prefill of one sequence of token ids (S,); returns the last position's logits (vocab,)
@@ -128,15 +183,9 @@ class TPLlamaPrefill:
         S, D = tokens.shape[0], cfg.head_dim
         cos, sin = rope_tables(S, D, cfg.rope_base, self.device)
         x = self.embed[tokens]
-        nq, nk = self.hq_l * D, self.hk_l * D
         attn = torch.empty(1, S, self.hq_l, D, device=self.device, dtype=self.dtype)
-        for L in self.layers:
-            h = rms_norm(x, L["attn_norm"], cfg.eps)
-            qkv = h @ L["wqkv"].t()
-            q = apply_rope(qkv[:, :nq].view(S, self.hq_l, D), cos, sin)
-            k = apply_rope(qkv[:, nq:nq + nk].view(S, self.hk_l, D), cos, sin)
-            v = qkv[:, nq + nk:].view(S, self.hk_l, D)
-            del qkv
+
+        def attend(q, k, v):
             if events is not None:
                 e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
                 e0.record()
@@ -144,20 +193,86 @@ class TPLlamaPrefill:
             if events is not None:
                 e1.record()
                 events.append((e0, e1))
-            del q, k, v
-            o = attn.view(S, nq) @ L["wo"].t()
-            x = x + self._reduce(o)
-            del o
-            h = rms_norm(x, L["mlp_norm"], cfg.eps)
-            gu = h @ L["wgu"].t()
-            a = torch.nn.functional.silu(gu[:, :self.f_l]) * gu[:, self.f_l:]
-            del gu
-            y = a @ L["wd"].t()
-            del a
-            x = x + self._reduce(y)
-            del y
-        last = rms_norm(x[-1:], self.final_norm, cfg.eps)
-        return (last.float() @ self.lm_head.float().t())[0]
+            return attn.view(S, self.hq_l * D)
+
+        for L in self.layers:
+            x = self._layer(L, x, cos, sin, attend)
+        return self._logits(x[-1:])[0]
+
+    # ------------------------------------------------------------------ with a paged cache (CUDA only)
+    def new_cache(self, batch: int, max_len: int, page_size: int = 64, dtype: torch.dtype | None = None) -> LlamaCache:
+        """An empty cache for ``batch`` sequences of up to ``max_len`` tokens; ``dtype``: the model's, or
+        torch.float8_e4m3fn."""
+        from .paged_cache import kv_cache_alloc
+        pages = -(-max_len // page_size)
+        layers = [kv_cache_alloc(batch * pages, page_size, self.hk_l, dtype or self.dtype, self.device) for _ in self.layers]
+        table = torch.arange(batch * pages, dtype=torch.int32, device=self.device).view(batch, pages)
+        return LlamaCache(layers, table, torch.zeros(batch, dtype=torch.int32, device=self.device), [0] * batch,
+                          rope_tables(pages * page_size, self.cfg.head_dim, self.cfg.rope_base, self.device))
+
+    @torch.no_grad()
+    def prefill(self, tokens: torch.Tensor, cache: LlamaCache, seq: int = 0) -> torch.Tensor:
+        """Append the token ids (S,) to sequence ``seq`` of the cache and return the last one's logits (vocab,) in fp32.
+        Tokens after the first chunk attend to the cached prefix, read back, and to their own keys."""
+        from .paged_cache import kv_cache_read, kv_cache_write
+        cfg = self.cfg
+        S, D, n = tokens.shape[0], cfg.head_dim, cache.lens[seq]
+        if S < 1 or n + S > cache.max_len:
+            raise ValueError(f"{S} tokens after {n} do not fit the cache's {cache.max_len}")
+        pos = torch.arange(n, n + S, device=self.device)
+        slots = cache.slots(torch.full_like(pos, seq), pos)
+        cos, sin = (t[n:n + S] for t in cache.rope)
+        x = self.embed[tokens]
+        attn = torch.empty(1, S, self.hq_l, D, device=self.device, dtype=self.dtype)
+        whole = [torch.empty(1, n + S, self.hk_l, D, device=self.device, dtype=self.dtype) for _ in range(2)] if n else None
+        layers = iter(cache.layers)
+
+        def attend(q, k, v):
+            c = next(layers)
+            if n:
+                kw, vw = whole
+                kv_cache_read(c.k, c.v, cache.page_table[seq:seq + 1], cache.seq_lens[seq:seq + 1], kw, vw, c.k_scale,
+                              c.v_scale)
+                kw[0, n:], vw[0, n:] = k, v
+            self.attention(q[None], whole[0] if n else k[None], whole[1] if n else v[None], attn, cfg)
+            kv_cache_write(k, v, c.k, c.v, slots, c.k_scale, c.v_scale)
+            return attn.view(S, self.hq_l * D)
+
+        for L in self.layers:
+            x = self._layer(L, x, cos, sin, attend)
+        cache.lens[seq] = n + S
+        cache.seq_lens[seq] = n + S
+        return self._logits(x[-1:])[0]
+
+    @torch.no_grad()
+    def decode(self, tokens: torch.Tensor, cache: LlamaCache) -> torch.Tensor:
+        """One new token id for each sequence of the cache, (batch,); returns the logits (batch, vocab) in fp32."""
+        from .paged_cache import kv_cache_write, paged_decode
+        cfg = self.cfg
+        B, D = tokens.shape[0], cfg.head_dim
+        if B != len(cache.lens):
+            raise ValueError(f"{B} tokens for the cache's {len(cache.lens)} sequences")
+        if max(cache.lens) >= cache.max_len:
+            raise ValueError(f"a sequence fills the cache's {cache.max_len} tokens")
+        pos = cache.seq_lens.long()
+        slots = cache.slots(torch.arange(B, device=self.device), pos)
+        cos, sin = (t[pos] for t in cache.rope)
+        lens = cache.seq_lens + 1
+        x = self.embed[tokens]
+        layers = iter(cache.layers)
+
+        def attend(q, k, v):
+            c = next(layers)
+            kv_cache_write(k, v, c.k, c.v, slots, c.k_scale, c.v_scale)
+            out = torch.empty_like(q)
+            paged_decode(q, c.k, c.v, cache.page_table, lens, out, None, c.k_scale, c.v_scale)
+            return out.view(B, self.hq_l * D)
+
+        for L in self.layers:
+            x = self._layer(L, x, cos, sin, attend)
+        cache.seq_lens += 1
+        cache.lens = [n + 1 for n in cache.lens]
+        return self._logits(x)
 
 
 def _flash_prefill_attention(q, k, v, out, cfg: LlamaConfig):

@@ -1,5 +1,6 @@
-"""The operator as registered PyTorch ops: ``torch.ops.flashprefill.prefill_dense`` and
-``torch.ops.flashprefill.prefill_varlen``.
+"""The operators as registered PyTorch ops: ``torch.ops.flashprefill.prefill_dense`` and
+``torch.ops.flashprefill.prefill_varlen``, and for the paged cache ``kv_cache_write``, ``kv_cache_read`` and
+``paged_decode`` of the same namespace.
 
 They wrap the same C ABI entry points as ``flash_prefill`` / ``flash_prefill_varlen_func``
 (``fpb_prefill_dense`` / ``fpb_prefill_varlen``), each writing its output argument in place.
@@ -8,6 +9,8 @@ tracing can follow a model that calls them without a graph break.  The reference
 Python functions directly; these ops take the same positional arguments.
 """
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 
@@ -42,4 +45,44 @@ def prefill_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.T
 @prefill_varlen.register_fake
 def _(q, k, v, o, cu_seqlens, max_seq_len, alpha, block_size=128, attention_sink=2, window_size=4,
       last_n_block=2):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::kv_cache_write", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"),
+                         device_types="cuda")
+def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                   k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor]) -> None:
+    """paged_cache.kv_cache_write as a registered op (what it writes is given: None scales for a 16-bit cache)."""
+    _ops.kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
+
+
+@kv_cache_write.register_fake
+def _(k, v, k_cache, v_cache, slots, k_scale, v_scale):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::kv_cache_read", mutates_args=("k", "v"), device_types="cuda")
+def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                  k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                  v_scale: Optional[torch.Tensor] = None) -> None:
+    """paged_cache.kv_cache_read as a registered op."""
+    _ops.kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale)
+
+
+@kv_cache_read.register_fake
+def _(k_cache, v_cache, page_table, seq_lens, k, v, k_scale=None, v_scale=None):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::paged_decode", mutates_args=("out", "lse"), device_types="cuda")
+def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                 seq_lens: torch.Tensor, out: torch.Tensor, lse: Optional[torch.Tensor],
+                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                 sm_scale: Optional[float] = None) -> None:
+    """paged_cache.paged_decode as a registered op (its workspace from the caching allocator)."""
+    _ops.paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale, None)
+
+
+@paged_decode.register_fake
+def _(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale=None, v_scale=None, sm_scale=None):
     return None
