@@ -19,7 +19,7 @@ _DTYPES = {torch.bfloat16: _lib.FPB_BF16, torch.float16: _lib.FPB_FP16}
 # (the reference's autotuner picks 4 or 8, ops/flashprefill_native_forward.py:7-20).
 _MEAN_WARPS = int(os.environ.get("FLASHPREFILL_B200_MEAN_WARPS", "4"))
 # When set, every call synchronises and raises if a kernel reported a device error.
-_CHECK = os.environ.get("FLASHPREFILL_B200_CHECK", "0") not in ("", "0")
+CHECK = _CHECK = os.environ.get("FLASHPREFILL_B200_CHECK", "0") not in ("", "0")
 
 LAYOUT_KEYS = ["err", "cu_tile", "mk", "cnt", "idx", "total", "tiles", "cap"]
 
@@ -333,30 +333,15 @@ def check_paged_error(device=None) -> None:
     _lib.check(rc)
 
 
-def _finish_paged(device) -> None:
-    if _CHECK and not torch.cuda.is_current_stream_capturing():
-        check_paged_error(device)
-
-
-# The entry points' checks and launches are in csrc/fp_torch.cpp.
-def kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale) -> None:
-    (_lib._ext or _lib.ext()).kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
-    if _CHECK and not torch.cuda.is_current_stream_capturing():
+def finish_paged(device, slots=None) -> None:
+    """After a paged-cache call with FLASHPREFILL_B200_CHECK set: raise what it met on the device."""
+    if torch.cuda.is_current_stream_capturing():
+        return
+    if slots is not None:
         used = slots[slots >= 0]
         if used.unique().numel() != used.numel():
             raise ValueError("two rows name one slot")
-        check_paged_error(k.device)
-
-
-def kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale) -> None:
-    (_lib._ext or _lib.ext()).kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale)
-    _finish_paged(k.device)
-
-
-def paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale, workspace) -> None:
-    (_lib._ext or _lib.ext()).paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale,
-                                           workspace)
-    _finish_paged(q.device)
+    check_paged_error(device)
 
 
 def paged_decode_workspace_bytes(batch, q_heads, kv_heads, cache_dtype, max_pages, page_size) -> int:

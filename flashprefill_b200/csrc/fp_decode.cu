@@ -76,8 +76,14 @@ struct DecodeArgs {
   float2* ml;                        // [2 * piece + slot][nh] {maximum (log2 units), sum}
 };
 
+// 16 bytes of the cache (`bytes` of them, then zeros) to shared memory.  Cached rows pass through L2 once: evicted first, they
+// leave it to the tables, lengths and partial sums (28/4 heads, 33 x up to 16001 tokens of e4m3: 57 us without, 53 with).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes),
+               "l"(policy)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

@@ -111,14 +111,14 @@ void head_groups(int G, int* ngroups, int* nh) {
 // How a call runs.  Every size here is a bound from the table's width: lengths are known on the device only.
 //
 // Short sequences: a cluster for each item, if no warp gets more than kShortTiles tiles that way: as many CTAs as the GPU holds
-// at once, 8 at most.  Few items of more than kNarrowTiles tiles a warp take wide CTAs, so that a warp's tiles, one after
-// another, are fewer (32/8 heads, bf16: 1 x 4096 tokens 12.7 us with 4 warps, 9.3 with 12; 2 x 1024, 2 tiles a warp, 6.9 and 7.9).
+// at once, 8 at most; wide CTAs where a warp's tiles, one after another, are fewer that way (32/8 heads, bf16: 1 x 4096 tokens
+// 12.7 us with 8 x 4 warps an item, 9.3 with 8 x 12; 2 x 1024, 2 tiles a warp either way, 6.9 and 7.9).
 // Else pieces of the line of all units: 8192 tokens of one such sequence take 20 us in clusters of narrow CTAs, 15 in
 // pieces, 13 in clusters of wide ones; 256 x up to 600 tokens of 8/2 heads 20 in clusters and 22 in pieces.  Few items, each of several
 // pieces, take wide CTAs, which leave a third as many partial sums (2 x 262144 tokens, 28/4 heads, e4m3: 92 and 90 us); many
 // ragged ones narrow CTAs, which wait for one another less (64 x up to 8192: 171 and 174).
 constexpr int kSms = 148;
-constexpr int kShortTiles = 12, kNarrowTiles = 3;
+constexpr int kShortTiles = 12;
 struct DecodeShape {
   int G, ngroups, nh;
   int warps, cluster;    // of a CTA; cluster 0: pieces
@@ -133,20 +133,27 @@ DecodeShape decode_shape(int batch, int hq, int hk, int cache_dtype, int max_pag
   const int nt = s.nh <= 8 ? 1 : 2, tile = cache_dtype == FPB_E4M3 ? 32 : 16;
   const int64_t tiles = ((int64_t)max_pages * page_size + tile - 1) / tile;
   s.items = (int64_t)batch * hk * s.ngroups;
-  s.warps = s.items <= kSms && tiles > kNarrowTiles * kNarrow * kDecMaxCluster ? wide_warps(nt) : kNarrow;
-  const int64_t units = (tiles + s.warps - 1) / s.warps, places = kSms * dec_ctas_per_sm(nt, s.warps);
-  s.cluster = 1;
-  while (s.cluster < kDecMaxCluster && 2 * s.cluster <= units && s.items * 2 * s.cluster <= places) s.cluster *= 2;
-  if (tiles > (int64_t)kShortTiles * s.warps * s.cluster || s.items * s.cluster >= (int64_t(1) << 31)) {
+  // the largest cluster of CTAs of `warps` warps that fits with all others, and the tiles of a warp
+  auto cluster = [&](int warps) {
+    const int64_t units = (tiles + warps - 1) / warps, places = kSms * dec_ctas_per_sm(nt, warps);
+    int c = 1;
+    while (c < kDecMaxCluster && 2 * c <= units && s.items * 2 * c <= places) c *= 2;
+    return c;
+  };
+  auto each_warp = [&](int warps) { return (tiles + warps * cluster(warps) - 1) / (warps * cluster(warps)); };
+  const int wide = wide_warps(nt);
+  s.warps = s.items <= kSms && each_warp(wide) < each_warp(kNarrow) ? wide : kNarrow;
+  s.cluster = cluster(s.warps);
+  if (each_warp(s.warps) > kShortTiles || s.items * s.cluster >= (int64_t(1) << 31)) {
     s.cluster = 0;
-    s.warps = 2 * s.items <= kSms ? wide_warps(nt) : kNarrow;
+    s.warps = 2 * s.items <= kSms ? wide : kNarrow;
   }
   s.units = s.items * ((tiles + s.warps - 1) / s.warps + 1);
   s.pieces = (int)std::min<int64_t>(kSms * dec_ctas_per_sm(nt, s.warps), s.units);
   s.by_item = s.items <= s.pieces;
   // heads share a CTA of the join where an item has few pieces, and have one each where it has many
-  const int64_t each = s.pieces / s.items;
-  s.join_heads = each >= 16 ? 1 : each >= 2 ? std::min(s.nh, 2) : std::min(s.nh, kJoinThreads / 32);
+  const int64_t pieces_each = s.pieces / s.items;
+  s.join_heads = pieces_each >= 16 ? 1 : pieces_each >= 2 ? std::min(s.nh, 2) : std::min(s.nh, kJoinThreads / 32);
   return s;
 }
 int decode_descs(const DecodeShape& s) { return s.by_item ? (int)s.items : s.pieces; }

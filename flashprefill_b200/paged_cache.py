@@ -21,7 +21,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _ops
+from . import _lib, _ops
 
 
 class KVCache(NamedTuple):
@@ -55,7 +55,9 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     a NaN reads back as NaN.  k and v may have any strides (e.g. columns of a fused projection; copied only where rows are not
     16-byte aligned).  The slots of one call must differ from one another (FLASHPREFILL_B200_CHECK=1 checks that); where two
     rows name one slot, its contents are not defined."""
-    _ops.kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
+    (_lib._ext or _lib.ext()).kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
+    if _ops.CHECK:
+        _ops.finish_paged(k.device, slots)
 
 
 def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -65,7 +67,9 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torc
     ``flash_prefill`` takes for a cached prefix, dequantising an e4m3 cache to their 16-bit type.  Rows from ``seq_lens[b]`` on
     are left as they were, as is all of a sequence whose length is outside [0, S].  page_table (B, P) and seq_lens (B,) are
     int32."""
-    _ops.kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale)
+    (_lib._ext or _lib.ext()).kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale)
+    if _ops.CHECK:
+        _ops.finish_paged(k.device)
 
 
 def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -80,4 +84,7 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     1/sqrt(128) by default.  ``workspace``: uint8 of at least ``paged_decode_workspace_bytes``, taken from the caching
     allocator by default; calls that may overlap on the GPU (other streams, graphs replayed side by side) need one each.
     Results do not depend on the order in which the GPU runs its blocks: the same call gives the same bits."""
-    _ops.paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale, workspace)
+    (_lib._ext or _lib.ext()).paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale,
+                                           workspace)
+    if _ops.CHECK:
+        _ops.finish_paged(q.device)

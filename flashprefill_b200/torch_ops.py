@@ -14,7 +14,7 @@ from typing import Optional
 
 import torch
 
-from . import _ops
+from . import _ops, paged_cache
 
 _NS = "flashprefill"
 
@@ -53,7 +53,7 @@ def _(q, k, v, o, cu_seqlens, max_seq_len, alpha, block_size=128, attention_sink
 def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
                    k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor]) -> None:
     """paged_cache.kv_cache_write as a registered op (what it writes is given: None scales for a 16-bit cache)."""
-    _ops.kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
+    paged_cache.kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
 
 
 @kv_cache_write.register_fake
@@ -66,7 +66,7 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torc
                   k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                   v_scale: Optional[torch.Tensor] = None) -> None:
     """paged_cache.kv_cache_read as a registered op."""
-    _ops.kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale)
+    paged_cache.kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale)
 
 
 @kv_cache_read.register_fake
@@ -80,7 +80,7 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
                  k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
                  sm_scale: Optional[float] = None) -> None:
     """paged_cache.paged_decode as a registered op (its workspace from the caching allocator)."""
-    _ops.paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale, None)
+    paged_cache.paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale)
 
 
 @paged_decode.register_fake
