@@ -1,8 +1,8 @@
 // Tensor plumbing of the paged-cache entry points: checks, strides, workspace and stream, then the C ABI of
 // libflashprefill_b200.so (include/flashprefill_b200.h), whose functions are handed over by address at load time.
 //
-// These calls run once for each layer of each token, and the small ones take 2 to 8 us on the GPU; the same plumbing in
-// Python through ctypes took 20 to 34 us a call, so it bound every call below 200 MB of cache.  It is plain CPython
+// These calls run once for each layer of each token, and the small ones take 1.5 to 5 us on the GPU; the same plumbing in
+// Python through ctypes took 20 to 34 us a call, so it bound every call below 200 MB of cache; this takes 3 to 4.  It is plain CPython
 // (vectorcall) over torch's C++ tensors.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -170,6 +170,7 @@ void write_(PyObject* const* a) {
   REFUSE(v.sizes() != k.sizes(), Value, "v shape ", v.sizes(), " must equal k shape ", k.sizes());
   REFUSE(v.scalar_type() != k.scalar_type(), Type, "k and v must share one dtype");
   const Cache c = cache_args(a[2], a[3], a[5], a[6], k, device, k.size(1), true);
+  REFUSE(c.k->data_ptr() == c.v->data_ptr(), Value, "k_cache and v_cache must not be the same memory");
   const at::Tensor& s = tensor(a[4], "slots", 1, &device);
   REFUSE(s.scalar_type() != at::kLong && s.scalar_type() != at::kInt, Type, "slots must be int64 or int32, got ", s.scalar_type());
   REFUSE(s.size(0) != k.size(0), Value, "slots must have one entry for each of the ", k.size(0), " rows, got ", s.size(0));
@@ -193,6 +194,7 @@ void read_(PyObject* const* a) {
     REFUSE(t->numel() && !rows_ok(*t), Value, t == &k ? "k" : "v", " must have a contiguous last dimension and 16-byte aligned rows");
   }
   REFUSE(v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type(), Value, "k and v must share shape and dtype");
+  REFUSE(k.numel() && k.data_ptr() == v.data_ptr(), Value, "k and v must not be the same memory");
   const Cache c = cache_args(a[0], a[1], a[6], a[7], k, device, k.size(2), false);
   const Table t = table_args(a[2], a[3], k.size(0), device);
   if (k.size(0) == 0 || k.size(1) == 0 || t.width == 0) return;

@@ -228,6 +228,8 @@ def test_write_of_extreme_rows(dtype):
 @pytest.mark.parametrize("lens,hk,ps,layout", [
     ([1], 1, 16, "hnd"), ([0, 5, 16, 17], 8, 16, "nhd"), ([300, 0, 129], 3, 48, "hnd"), ([1, 2, 3], 2, 1, "nhd"),
     ([2050], 4, 128, "hnd"),
+    # calls large enough for the kernel that takes 4 tokens at a time, where 4 divides page_size
+    ([3001, 0, 2998, 4099], 8, 16, "nhd"), ([2, 4099, 4098, 4097], 5, 4, "hnd"), ([4099, 3, 4096, 4000], 5, 6, "nhd"),
 ])
 def test_read_matches_the_definition(lens, hk, ps, layout, quant, dtype):
     f = pu.fill_sequences(lens, hk, hk, dtype, E4M3 if quant else dtype, ps, layout, seed=len(lens))
@@ -244,12 +246,14 @@ def test_read_matches_the_definition(lens, hk, ps, layout, quant, dtype):
 
 
 # ------------------------------------------------------------------ decode
-def check_decode(f, out, lse, dtype, cache_dtype, sm_scale=128 ** -0.5):
+def check_decode(f, out, lse, dtype, cache_dtype, sm_scale=128 ** -0.5, lse_too=True):
     for b, (k, v) in enumerate(f["rows"]):
         ref, rl, weight, size = pu.attend64(f["q"][b], k, v, sm_scale)
         to, tl = pu.decode_bounds(ref, rl, weight, size, k.shape[0], dtype, cache_dtype, f["q"][b], k, v, sm_scale)
         err = (out[b].double() - ref).abs()
         assert (err <= to).all(), (b, k.shape[0], (err / to.clamp_min(1e-30)).max().item())
+        if not lse_too:
+            continue
         if k.shape[0] == 0:
             assert (lse[b] == -float("inf")).all()
         else:
@@ -270,6 +274,8 @@ DECODE_CASES = [  # lens, q heads, kv heads, page size, layout
     ([40000], 4, 1, 256, "nhd"),
     ([20000, 0, 3, 9000, 65, 17001], 8, 2, 64, "hnd"),
     ([100] * 150, 8, 2, 16, "nhd"),
+    ([70, 0, 9, 300] * 10, 24, 2, 32, "hnd"),  # 12 heads a KV head, more items than half the SMs
+    ([2000, 5], 128, 4, 16, "nhd"),            # 32 heads a KV head
 ]
 
 
@@ -522,14 +528,15 @@ def test_python_refusals():
         ((rows[:, :1], rows[:, :1], k, v, slots, ks, vs), ValueError, "KV heads"), ((rows, rows, k, v, slots[:2], ks, vs), ValueError, "slots"),
         ((rows, rows, k, v, slots.float(), ks, vs), TypeError, "slots"), ((rows, rows, k, v, slots[None], ks, vs), ValueError, "dimensions"),
         ((rows, rows, k[:1].expand_as(k), v[:1].expand_as(v), slots, ks, vs), ValueError, "expanded"),
+        ((rows, rows, k, k, slots, ks, vs), ValueError, "same memory"),
     ]:
         with pytest.raises(err, match=msg):
             fp.kv_cache_write(*a)
-    to = torch.zeros(2, 40, 2, 128, dtype=BF16, device="cuda")
+    to, to2 = (torch.zeros(2, 40, 2, 128, dtype=BF16, device="cuda") for _ in range(2))
     for a, err, msg in [
         ((k, v, t, n, to, to[:, :20], ks, vs), ValueError, "share"), ((k, v, t, n, to[..., ::2], to[..., ::2], ks, vs), ValueError, "contiguous"),
-        ((k, v, t, n, to.float(), to.float(), ks, vs), TypeError, "bfloat16"), ((k, v, t[:1], n, to, to, ks, vs), ValueError, "rows"),
-        ((k, v, t, n, to[:, :1].expand_as(to), to, ks, vs), ValueError, "expanded"),
+        ((k, v, t, n, to.float(), to.float(), ks, vs), TypeError, "bfloat16"), ((k, v, t[:1], n, to, to2, ks, vs), ValueError, "rows"),
+        ((k, v, t, n, to[:, :1].expand_as(to), to, ks, vs), ValueError, "expanded"), ((k, v, t, n, to, to, ks, vs), ValueError, "same memory"),
     ]:
         with pytest.raises(err, match=msg):
             fp.kv_cache_read(*a)
@@ -545,3 +552,82 @@ def test_empty_calls_do_nothing():
     fp.paged_decode(none, *c[:2], table, lens, torch.empty_like(none))
     fp.kv_cache_read(*c[:2], table, lens, none[:, None], none[:, None])
     fp.check_paged_error()
+
+
+@pytest.mark.gpu
+def test_two_threads_on_streams_of_their_own():
+    """Calls from two threads at once, each on its own stream with a workspace from the allocator: each gets its own result."""
+    import threading
+    fs = [pu.fill_sequences([9000 + 50 * i, 130, 0], 8, 2, BF16, E4M3 if i else BF16, 16, seed=20 + i, room=60000) for i in range(2)]
+    want = []
+    for f in fs:
+        o = torch.empty_like(f["q"])
+        fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], o, None, f["k_scale"], f["v_scale"])
+        want.append(o)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        f = fs[i]
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                o = torch.empty_like(f["q"])
+                fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], o, None, f["k_scale"], f["v_scale"])
+                if not same_bits(o, want[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+    fp.check_paged_error()
+
+
+@pytest.mark.gpu
+def test_a_call_waits_for_what_the_stream_holds():
+    """Rows written, read and attended to in one go behind a long kernel, many times over: no call may see what its predecessors
+    on the stream have not finished (its launch is prepared while they run)."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    big = torch.randn(4096, 4096, generator=g, device="cuda", dtype=BF16)
+    cache = fp.kv_cache_alloc(64, 16, 2)
+    table = torch.arange(64, dtype=torch.int32, device="cuda")[None]
+    n = 1000
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    slots = torch.arange(n, device="cuda")
+    q = torch.randn(1, 8, 128, generator=g, device="cuda").to(BF16)
+    for i in range(20):
+        k, v = (torch.randn(n, 2, 128, generator=g, device="cuda").to(BF16) for _ in range(2))
+        torch.cuda.synchronize()
+        big @ big
+        late_k, late_v = k * 1.0, v * 1.0  # made on the stream just before the write
+        kr, vr, out = torch.empty(1, n, 2, 128, dtype=BF16, device="cuda"), torch.empty(1, n, 2, 128, dtype=BF16, device="cuda"), torch.empty_like(q)
+        fp.kv_cache_write(late_k, late_v, cache.k, cache.v, slots)
+        fp.paged_decode(q, cache.k, cache.v, table, lens, out)
+        fp.kv_cache_read(cache.k, cache.v, table, lens, kr, vr)
+        after = out + 0  # and nothing behind a call may run ahead of it
+        torch.cuda.synchronize()
+        assert same_bits(kr[0], k) and same_bits(vr[0], v)
+        check_decode(dict(q=q, rows=[[k.double(), v.double()]]), after, torch.full((1, 8), float("nan"), device="cuda"), BF16, BF16, lse_too=False)
+
+
+@pytest.mark.gpu
+def test_checked_mode_raises_from_the_call(tmp_path):
+    """FLASHPREFILL_B200_CHECK=1 (read at import): two rows for one slot and a slot outside the cache raise from the call."""
+    import subprocess
+    import sys
+    code = """
+import torch, flashprefill_b200 as fp
+c = fp.kv_cache_alloc(4, 16, 1)
+r = torch.zeros(2, 1, 128, dtype=torch.bfloat16, device="cuda")
+fp.kv_cache_write(r, r, c.k, c.v, torch.tensor([3, 4], device="cuda"))
+for slots, err in (([5, 5], ValueError), ([1, 64], fp.FlashPrefillError)):
+    try:
+        fp.kv_cache_write(r, r, c.k, c.v, torch.tensor(slots, device="cuda"))
+    except err as e:
+        print(type(e).__name__)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, FLASHPREFILL_B200_CHECK="1", PYTHONPATH=root), capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split() == ["ValueError", "FlashPrefillError"], r.stdout + r.stderr
