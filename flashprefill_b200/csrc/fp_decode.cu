@@ -7,14 +7,14 @@
 // KV head share its rows.  Each cached byte is read once and meets G flops (2-byte cache) or 2 G (e4m3), so the operator is
 // bound by HBM; the arithmetic only has to stay out of the way.
 //
-// An item is (sequence, KV head, group of query heads: all G up to 16, equal groups of at most 16 above that), its tokens are cut
-// into units of TT tokens for each warp of a CTA.  Lengths are read on the device (no host copy; a captured graph serves any lengths).
+// An item is (sequence, KV head, group of query heads: all G up to 16, equal groups of at most 16 above that); its tokens are
+// cut into units of TT tokens for each warp of a CTA.  Lengths are read on the device (no host copy; a captured graph serves
+// any lengths).
 //
 // Long sequences (paged_decode_kernel).  All items' units form one line, with one empty unit at the head of each item for
 // what starting an item costs, and each of the CTAs that the GPU holds takes an equal piece of it, so ragged batches and
 // single long sequences load the GPU alike.  A piece that covers a whole item writes its output; an item cut between pieces
-// leaves unnormalised sums and their maxima in the workspace, which a second kernel (programmatic dependent launch) joins in
-// the order of the tokens.
+// leaves unnormalised sums and their maxima in the workspace; a second kernel joins them in the order of the tokens.
 // Short sequences (paged_decode_short_kernel): one cluster of 1 to 8 CTAs for each item, units dealt out in turn, joined
 // through distributed shared memory.  No prefix sums, no workspace, no second kernel.
 // Both join in an order that the lengths alone decide, with no atomics: the same call gives the same bits.
@@ -38,6 +38,12 @@
 //   * e4m3: codes widen to fp16 exactly; q is scaled by a power of two to fit fp16; the token's K scale multiplies its
 //     score and its V scale its weight, relative to the largest V scale so far (a running reference like the maximum), so
 //     weights stay at most 2^15.
+//
+// Measured (device time; of the measured 6.54 TB/s): 64 x up to 8192 tokens of 32/8 heads, bf16, 1.11 GB, 163 to 171 us (100%
+// and more: reads alone pass a copy's rate); 1 x 131072, 0.54 GB, 85 us (97%); 2 x up to 262144 of 28/4 heads, e4m3, 0.53 GB,
+// 83 to 88 us (92 to 98%), 46% of the issue slots; 33 x up to 16001 of 28/4 heads, e4m3, 0.31 GB, 53 to 57 us (82 to 88%): 3 us from
+// the launch to the first full stream (lengths, table, rows: three loads in turn), 3 us between the first CTA that ends and the
+// last, 4 us for the join.  1 x 500 of 32/8 heads, 2 MB, 4.5 us: the same loads in turn.
 #include <type_traits>
 
 #include "fp_common.cuh"

@@ -112,11 +112,11 @@ void head_groups(int G, int* ngroups, int* nh) {
 //
 // Short sequences: a cluster for each item, if no warp gets more than kShortTiles tiles that way: as many CTAs as the GPU holds
 // at once, 8 at most; wide CTAs where a warp's tiles, one after another, are fewer that way (32/8 heads, bf16: 1 x 4096 tokens
-// 12.7 us with 8 x 4 warps an item, 9.3 with 8 x 12; 2 x 1024, 2 tiles a warp either way, 6.9 and 7.9).
-// Else pieces of the line of all units: 8192 tokens of one such sequence take 20 us in clusters of narrow CTAs, 15 in
-// pieces, 13 in clusters of wide ones; 256 x up to 600 tokens of 8/2 heads 20 in clusters and 22 in pieces.  Few items, each of several
-// pieces, take wide CTAs, which leave a third as many partial sums (2 x 262144 tokens, 28/4 heads, e4m3: 92 and 90 us); many
-// ragged ones narrow CTAs, which wait for one another less (64 x up to 8192: 171 and 174).
+// 12.1 us with 8 x 4 warps an item, 9.0 with 8 x 12; 1 x 500, one tile a warp either way, 4.5 and 6.3).
+// Else pieces of the line of all units.  Clusters win up to there (1 x 8192 tokens 12.4 us, 13.3 in pieces; 256 x up to 600 of
+// 8/2 heads 19.7 and 21.4) and lose beyond (8 x up to 32000 of 48/4 heads, e4m3, 54 us and 42 in pieces).  Few items, each of
+// several pieces, take wide CTAs, which leave a third as many partial sums (2 x up to 262144 tokens of 28/4 heads, e4m3: 82.8 us,
+// narrow 84.1); many ragged ones narrow CTAs, which wait for one another less (64 x up to 1024 of 32/8: 28.3 us, wide 33.1).
 constexpr int kSms = 148;
 constexpr int kShortTiles = 12;
 struct DecodeShape {
@@ -151,9 +151,8 @@ DecodeShape decode_shape(int batch, int hq, int hk, int cache_dtype, int max_pag
   s.units = s.items * ((tiles + s.warps - 1) / s.warps + 1);
   s.pieces = (int)std::min<int64_t>(kSms * dec_ctas_per_sm(nt, s.warps), s.units);
   s.by_item = s.items <= s.pieces;
-  // heads share a CTA of the join where an item has few pieces, and have one each where it has many
-  const int64_t pieces_each = s.pieces / s.items;
-  s.join_heads = pieces_each >= 16 ? 1 : pieces_each >= 2 ? std::min(s.nh, 2) : std::min(s.nh, kJoinThreads / 32);
+  // an item of many pieces has a CTA of the join for each head (2 x up to 262144 tokens of 28/4 heads: 82.8 us, 86.4 without)
+  s.join_heads = s.pieces / s.items >= 16 ? 1 : std::min(s.nh, kJoinThreads / 32);
   return s;
 }
 int decode_descs(const DecodeShape& s) { return s.by_item ? (int)s.items : s.pieces; }
@@ -229,8 +228,8 @@ int fpb_kv_cache_read(const void* k_cache, const void* v_cache, int cache_dtype,
                      v_scale, scale_strides));
   FPB_TRY(check_table(page_table, table_stride, max_pages, page_size, seq_lens, batch));
   FPB_CHECK_ARG(batch <= 65535, "batch (%d) must be at most 65535", batch);
-  FPB_CHECK_ARG(out_len >= 1 && ((int64_t)out_len + 3) * hk < (int64_t(1) << 31) - 16, "out_len (%d) must be >= 1 and out_len * num_kv_heads below 2^31",
-                out_len);
+  FPB_CHECK_ARG(out_len >= 1 && ((int64_t)out_len + 3) * hk < (int64_t(1) << 31) - 16,
+                "out_len (%d) must be >= 1 and out_len * num_kv_heads below 2^31", out_len);
   FPB_TRY(check_ptr(k, "k"));
   FPB_TRY(check_ptr(v, "v"));
   FPB_TRY(check_strides(k_strides, 3, "k"));
@@ -279,7 +278,8 @@ int fpb_paged_decode(const void* q, int dtype, int batch, int hq, int hk, int he
   FPB_CHECK_ARG(std::isfinite(sm_scale), "sm_scale must be finite");
   const DecodeShape s = decode_shape(batch, hq, hk, cache_dtype, max_pages, page_size);
   if (s.cluster == 0) {
-    FPB_CHECK_ARG(s.units < (int64_t(1) << 31), "too many tokens for one call: batch * num_kv_heads * max_pages * page_size (narrow the page table)");
+    FPB_CHECK_ARG(s.units < (int64_t(1) << 31),
+                  "too many tokens for one call: batch * num_kv_heads * max_pages * page_size (narrow the page table)");
     FPB_CHECK_ARG(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                   "workspace must be a 256-byte aligned device pointer");
     FPB_CHECK_ARG((int64_t)workspace_bytes >= decode_ws_total(s), "workspace too small: %zu bytes given, %lld needed",
