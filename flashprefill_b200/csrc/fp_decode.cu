@@ -120,16 +120,18 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// First of a cluster's two barriers: every CTA has started, so its shared memory may be written from the others.
+__device__ __forceinline__ void cluster_started_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_started_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+// Second: what the CTAs wrote into one another is there.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Reads the float at this CTA's shared address `addr` in CTA `rank` of the cluster.
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+// Writes the float at this CTA's shared address `addr` in CTA `rank` of the cluster.
+__device__ __forceinline__ void st_cluster(uint32_t addr, int rank, float v) {
   uint32_t remote;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
@@ -670,65 +672,62 @@ __global__ void __launch_bounds__(kWarps * 32, dec_ctas_per_sm(NT, kWarps)) page
   }
 }
 
-// One item for each cluster of `cluster` CTAs (up to 8); CTA r takes the units r, r + cluster, ...
+// One item for each cluster of `cluster` CTAs (up to 8); CTA r takes the units r, r + cluster, ...  Head i is joined by CTA
+// i % cluster, into whose shared memory the others write their sums (written rather than fetched: one trip, and no CTA has to
+// stay for its readers).
 template <typename T, bool kE4m3, int NT, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, dec_ctas_per_sm(NT, kWarps)) paged_decode_short_kernel(const DecodeArgs A, int cluster) {
   using W = DecodeWarp<T, kE4m3, NT>;
   constexpr int kUnit = kWarps * W::TT;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 s_ml[kWarps][8 * NT];
-  __shared__ float s_x[8 * NT][kHeadDim];  // this CTA's sums, read by the others of the cluster
-  __shared__ float2 s_cta[8 * NT];
+  // sums and {maximum, sum} from CTA k of the heads that this one joins: row k * own + j is head rank + j * cluster
+  __shared__ float s_x[8 * NT + kDecMaxCluster][kHeadDim];
+  __shared__ float2 s_cta[8 * NT + kDecMaxCluster];
+  if (cluster > 1) cluster_started_arrive();
   await_stream();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = tid % kHeadDim;
   const int item = blockIdx.x / cluster, rank = blockIdx.x - item * cluster;
   const int HH = A.hk * A.ngroups, b = item / HH, hh = item - b * HH;
   const int h = hh / A.ngroups, grp = hh - h * A.ngroups;
   const int head0 = h * A.G + grp * A.nh, heads = min(A.nh, A.G - grp * A.nh);
+  const int own = (heads + cluster - 1) / cluster;  // heads of a CTA: cluster * own < heads + cluster rows
   W w;
   w.lane = lane;
   w.ring = smem_u32(smem) + warp * kDecRingBytes;
   w.run(A, b, h, head0, heads, rank * kUnit + warp * W::TT, cluster * kUnit, seq_len_of(A, b));
   w.store(reinterpret_cast<float*>(smem + warp * kDecRingBytes), s_ml[warp]);
   __syncthreads();
+  if (cluster > 1) cluster_started_wait();
   for (int i = tid / kHeadDim; i < heads; i += kWarps * 32 / kHeadDim) {
     float x, l, mx;
     merge_warps<kWarps, NT>(smem, s_ml, i, d, x, l, mx);
     if (cluster == 1) {
       write_head<T>(A, b, head0 + i, d, x, l, mx);
     } else {
-      s_x[i][d] = x;
-      if (d == 0) s_cta[i] = make_float2(mx, l);
+      const int j = i / cluster, to = i - j * cluster, row = rank * own + j;
+      st_cluster(smem_u32(&s_x[row][d]), to, x);
+      if (d == 0) {
+        st_cluster(smem_u32(&s_cta[row].x), to, mx);
+        st_cluster(smem_u32(&s_cta[row].y), to, l);
+      }
     }
   }
   if (cluster == 1) return;
   cluster_sync();
-  for (int i = rank + cluster * (tid / kHeadDim); i < heads; i += cluster * (kWarps * 32 / kHeadDim)) {
-    const uint32_t ax = smem_u32(&s_x[i][d]), am = smem_u32(&s_cta[i]);
-    float2 ml[kDecMaxCluster];
-    float xs[kDecMaxCluster], mx = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kDecMaxCluster; ++k) {
-      ml[k] = make_float2(-INFINITY, 0.f);
-      xs[k] = 0.f;
-      if (k < cluster) {
-        ml[k] = make_float2(ld_cluster(am, k), ld_cluster(am + 4, k));
-        xs[k] = ld_cluster(ax, k);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kDecMaxCluster; ++k) mx = fmaxf(mx, ml[k].x);
+  for (int j = tid / kHeadDim; rank + j * cluster < heads; j += kWarps * 32 / kHeadDim) {
+    float mx = -INFINITY;
+    for (int k = 0; k < cluster; ++k) mx = fmaxf(mx, s_cta[k * own + j].x);
     const float ref = finite_or_zero(mx);
     float l = 0.f, x = 0.f;
-#pragma unroll
-    for (int k = 0; k < kDecMaxCluster; ++k) {
-      const float f = ex2_approx(ml[k].x - ref);
-      l += f * ml[k].y;
-      x += f * xs[k];
+    for (int k = 0; k < cluster; ++k) {
+      const float2 ml = s_cta[k * own + j];
+      const float f = ex2_approx(ml.x - ref);
+      l += f * ml.y;
+      x += f * s_x[k * own + j][d];
     }
-    write_head<T>(A, b, head0 + i, d, x, l, mx);
+    write_head<T>(A, b, head0 + rank + j * cluster, d, x, l, mx);
   }
-  cluster_sync();  // no CTA leaves while others read its sums
 }
 
 __device__ __forceinline__ void scale4(float4& x, float f) { x = make_float4(x.x * f, x.y * f, x.z * f, x.w * f); }
