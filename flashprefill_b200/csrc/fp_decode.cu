@@ -52,13 +52,15 @@ namespace fpb {
 
 constexpr int kDecStages = 2;
 constexpr int kDecTileBytes = 4096;  // one warp's tile of K or of V
-constexpr int kDecRingBytes = kDecStages * 2 * kDecTileBytes;
+constexpr int kDecScaleBytes = 128;  // e4m3: scales of a tile's 32 rows of K or of V
+constexpr int kDecStageBytes = 2 * (kDecTileBytes + kDecScaleBytes);
+constexpr int kDecRingBytes = kDecStages * kDecStageBytes;
 // CTAs of narrow (4 warps) and wide form (as many as the registers hold: one CTA an SM), by 8s of heads of an item.
 constexpr int kNarrow = 4;
 constexpr int wide_warps(int nt) { return nt == 1 ? 12 : 8; }
 constexpr int dec_ctas_per_sm(int nt, int warps) { return wide_warps(nt) / warps; }
 constexpr int dec_smem_bytes(int warps) { return warps * kDecRingBytes; }
-constexpr int kDecMaxCluster = 8;
+constexpr int kDecMaxCluster = 8;  // clusters are powers of two: each divides the 8 NT heads of an item
 constexpr int kJoinThreads = 256;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -90,6 +92,14 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
   asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes),
                "l"(policy)
                : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float lds(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
+  return x;
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -239,14 +249,15 @@ struct DecodeWarp {
     }
   }
 
-  // Starts the copies of tokens [tok, tok + TT) below `end` into ring slot `stage`.  valid: bit r set where row r is there;
-  // ks, vs: the scales of this lane's token.
+  // Starts the copies of tokens [tok, tok + TT) below `end` into ring slot `stage`.  valid: bit r set where row r is there.
+  // The scales go to shared memory with the rows: loaded into registers a tile ahead, they were waited for together with
+  // the loads of the tile behind them (4 x 8100 tokens of 32/8 heads, e4m3: 18.3 us so, 17.0 this way).
   __device__ __forceinline__ void issue(const DecodeArgs& A, const int* table, int h, int tok, int end,
-                                        int stage, const int (&page)[MTILES], uint32_t& valid, float& ks, float& vs) {
+                                        int stage, const int (&page)[MTILES], uint32_t& valid) {
     constexpr int kRowsPer = 32 / kChunks;  // rows of one copy instruction of the warp
-    const uint32_t kd = ring + stage * 2 * kDecTileBytes, vd = kd + kDecTileBytes;
+    const uint32_t kd = ring + stage * kDecStageBytes, vd = kd + kDecTileBytes;
+    const uint32_t sd = kd + 2 * kDecTileBytes + 4 * lane;
     const int ch = lane % kChunks, r0 = lane / kChunks;
-    ks = vs = 0.f;
     if (A.page16) {
       valid = 0;
 #pragma unroll
@@ -276,10 +287,11 @@ struct DecodeWarp {
           vp += step;
         }
         if constexpr (kE4m3) {
-          if (lane / 16 == j && lane % 16 < rows) {
+          if (lane / 16 == j) {
             const uint64_t so = A.C.scales.at(pg, at + lane % 16, h);
-            ks = __ldg(A.C.k_scale + so);
-            vs = __ldg(A.C.v_scale + so);
+            const int bytes = lane % 16 < rows ? 4 : 0;
+            cp_async4(sd, A.C.k_scale + so, bytes);
+            cp_async4(sd + kDecScaleBytes, A.C.v_scale + so, bytes);
           }
         }
       }
@@ -287,18 +299,19 @@ struct DecodeWarp {
     }
     const int my = tok + lane % TT;
     int64_t off = -1;
+    uint64_t so = 0;
     if (my < end) {
       const int p = A.C.page_of(my), at = my - p * A.C.page_size, pg = __ldg(table + p);
       if ((unsigned)pg < (unsigned)A.C.num_pages) {
         off = (int64_t)(A.C.rows.at(pg, at, h) * 16);
-        if constexpr (kE4m3) {
-          const uint64_t so = A.C.scales.at(pg, at, h);
-          ks = __ldg(A.C.k_scale + so);
-          vs = __ldg(A.C.v_scale + so);
-        }
+        if constexpr (kE4m3) so = A.C.scales.at(pg, at, h);
       } else {
         raise_error(&g_paged_err, kErrBadPage);
       }
+    }
+    if constexpr (kE4m3) {
+      cp_async4(sd, A.C.k_scale + so, off < 0 ? 0 : 4);
+      cp_async4(sd + kDecScaleBytes, A.C.v_scale + so, off < 0 ? 0 : 4);
     }
     valid = __ballot_sync(0xffffffffu, off >= 0);
     if constexpr (TT == 16) valid &= 0xFFFFu;
@@ -307,15 +320,16 @@ struct DecodeWarp {
       const int r = i * kRowsPer + r0;
       const int64_t ro = __shfl_sync(0xffffffffu, off, r);
       const uint32_t d = r * kRowBytes + ((ch ^ (r & 7)) << 4);
-      const int64_t so = ro < 0 ? 0 : ro + ch * 16;
-      cp_async16(kd + d, A.C.k + so, ro < 0 ? 0 : 16);
-      cp_async16(vd + d, A.C.v + so, ro < 0 ? 0 : 16);
+      const int64_t src = ro < 0 ? 0 : ro + ch * 16;
+      cp_async16(kd + d, A.C.k + src, ro < 0 ? 0 : 16);
+      cp_async16(vd + d, A.C.v + src, ro < 0 ? 0 : 16);
     }
   }
 
-  __device__ __forceinline__ void consume(int stage, uint32_t valid, float ks, float vs) {
-    const uint32_t kd = ring + stage * 2 * kDecTileBytes, vd = kd + kDecTileBytes;
+  __device__ __forceinline__ void consume(int stage, uint32_t valid) {
+    const uint32_t kd = ring + stage * kDecStageBytes, vd = kd + kDecTileBytes;
     const int g = lane >> 2;
+    const uint32_t ksd = kd + 2 * kDecTileBytes, vsd = ksd + kDecScaleBytes;
     float s[NT][MTILES][4];
     {
       float s2[NT][4];  // second chain of products of a 16-token tile (32 tokens have two as it is)
@@ -364,7 +378,7 @@ struct DecodeWarp {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float kf = 1.f;
-        if constexpr (kE4m3) kf = __shfl_sync(0xffffffffu, ks, 16 * i + 8 * h + g);
+        if constexpr (kE4m3) kf = lds(ksd + 4 * (16 * i + 8 * h + g));
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -392,6 +406,7 @@ struct DecodeWarp {
         for (int i = 0; i < MTILES; ++i) mx[n][j] = fmaxf(mx[n][j], fmaxf(s[n][i][j], s[n][i][2 + j]));
         moved |= mx[n][j] > m[n][j];
       }
+    const float vs = kE4m3 ? lds(vsd + 4 * lane) : 0.f;
     if constexpr (kE4m3) moved |= !(vs <= vref);
     if (__any_sync(0xffffffffu, moved)) {
       float vcorr = 1.f;
@@ -422,13 +437,12 @@ struct DecodeWarp {
       }
     }
     uint32_t pb[NT][MTILES][2], pl[NT][MTILES][2];
-    const float vw = kE4m3 ? vs * vinv : 0.f;
 #pragma unroll
     for (int i = 0; i < MTILES; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float vf = 1.f;
-        if constexpr (kE4m3) vf = __shfl_sync(0xffffffffu, vw, 16 * i + 8 * h + g);
+        if constexpr (kE4m3) vf = lds(vsd + 4 * (16 * i + 8 * h + g)) * vinv;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float p[2];
@@ -474,7 +488,10 @@ struct DecodeWarp {
   }
 
   // All of this warp's tiles of an item: tokens [tok + i * step, + TT) below min(end, the sequence's length).  The first
-  // table entries and q are on their way before the length is needed.
+  // table entries and q are on their way before the length is needed.  kAhead: the next tile is asked for before, not after,
+  // the wait for this one.  That shortens a warp's chain of tiles (256 x up to 600 tokens 19.6 -> 18.2 us, 1 x 8192 11.6 -> 10.6) but puts
+  // more in flight than long streams bear (64 x up to 8192, bf16: 169 -> 176 us).
+  template <bool kAhead>
   __device__ __forceinline__ void run(const DecodeArgs& A, int b, int h, int head0, int heads, int tok, int step, int end) {
     const int* table = A.page_table + b * A.table_stride;
     int page[MTILES];
@@ -482,7 +499,6 @@ struct DecodeWarp {
     load_q(A, A.q + b * A.q_b + head0 * A.q_h, heads);
     const int n = end > tok ? (end - tok + step - 1) / step : 0;
     uint32_t valid[kDecStages];
-    float ks[kDecStages], vs[kDecStages];
 #pragma unroll
     for (int i = 0; i < kDecStages - 1; ++i) {
       if (i < n) {
@@ -490,7 +506,7 @@ struct DecodeWarp {
 #pragma unroll
         for (int j = 0; j < MTILES; ++j) cur[j] = page[j];
         if (i + 1 < n) load_pages(A, table, tok + (i + 1) * step, page);
-        issue(A, table, h, tok + i * step, end, i, cur, valid[i], ks[i], vs[i]);
+        issue(A, table, h, tok + i * step, end, i, cur, valid[i]);
       }
       cp_async_commit();
     }
@@ -500,19 +516,25 @@ struct DecodeWarp {
 #pragma unroll
       for (int j = 0; j < kDecStages; ++j) {
         if (i0 + j < n) {
-          cp_async_wait<kDecStages - 2>();
-          __syncwarp();
-          constexpr int kAhead = kDecStages - 1;
-          const int st = (j + kAhead) % kDecStages, nx = i0 + j + kAhead;
+          if constexpr (!kAhead) {
+            cp_async_wait<kDecStages - 2>();
+            __syncwarp();
+          }
+          constexpr int kNext = kDecStages - 1;
+          const int st = (j + kNext) % kDecStages, nx = i0 + j + kNext;
           if (nx < n) {
             int cur[MTILES];
 #pragma unroll
             for (int x = 0; x < MTILES; ++x) cur[x] = page[x];
             if (nx + 1 < n) load_pages(A, table, tok + (nx + 1) * step, page);
-            issue(A, table, h, tok + nx * step, end, st, cur, valid[st], ks[st], vs[st]);
+            issue(A, table, h, tok + nx * step, end, st, cur, valid[st]);
           }
           cp_async_commit();
-          consume(j, valid[j], ks[j], vs[j]);
+          if constexpr (kAhead) {
+            cp_async_wait<kDecStages - 1>();
+            __syncwarp();
+          }
+          consume(j, valid[j]);
           __syncwarp();
         }
       }
@@ -637,7 +659,7 @@ __global__ void __launch_bounds__(kWarps * 32, dec_ctas_per_sm(NT, kWarps)) page
     const int h = hh / A.ngroups, grp = hh - h * A.ngroups;
     const int head0 = h * A.G + grp * A.nh, heads = min(A.nh, A.G - grp * A.nh);
     // units u .. u_end hold the tokens [(u - 1) kUnit, (u_end - 1) kUnit); the first of an item none
-    w.run(A, b, h, head0, heads, max(u - 1, 0) * kUnit + warp * W::TT, kUnit,
+    w.template run<false>(A, b, h, head0, heads, max(u - 1, 0) * kUnit + warp * W::TT, kUnit,
           min(len, (u_end - 1) * kUnit));
     w.store(so, s_ml[warp]);
     __syncthreads();
@@ -672,7 +694,7 @@ __global__ void __launch_bounds__(kWarps * 32, dec_ctas_per_sm(NT, kWarps)) page
   }
 }
 
-// One item for each cluster of `cluster` CTAs (up to 8); CTA r takes the units r, r + cluster, ...  Head i is joined by CTA
+// One item for each cluster of `cluster` CTAs (1, 2, 4 or 8); CTA r takes the units r, r + cluster, ...  Head i is joined by CTA
 // i % cluster, into whose shared memory the others write their sums (written rather than fetched: one trip, and no CTA has to
 // stay for its readers).
 template <typename T, bool kE4m3, int NT, int kWarps>
@@ -682,8 +704,8 @@ __global__ void __launch_bounds__(kWarps * 32, dec_ctas_per_sm(NT, kWarps)) page
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 s_ml[kWarps][8 * NT];
   // sums and {maximum, sum} from CTA k of the heads that this one joins: row k * own + j is head rank + j * cluster
-  __shared__ float s_x[8 * NT + kDecMaxCluster][kHeadDim];
-  __shared__ float2 s_cta[8 * NT + kDecMaxCluster];
+  __shared__ float s_x[8 * NT][kHeadDim];
+  __shared__ float2 s_cta[8 * NT];
   if (cluster > 1) cluster_started_arrive();
   await_stream();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = tid % kHeadDim;
@@ -691,11 +713,11 @@ __global__ void __launch_bounds__(kWarps * 32, dec_ctas_per_sm(NT, kWarps)) page
   const int HH = A.hk * A.ngroups, b = item / HH, hh = item - b * HH;
   const int h = hh / A.ngroups, grp = hh - h * A.ngroups;
   const int head0 = h * A.G + grp * A.nh, heads = min(A.nh, A.G - grp * A.nh);
-  const int own = (heads + cluster - 1) / cluster;  // heads of a CTA: cluster * own < heads + cluster rows
+  const int own = (heads + cluster - 1) / cluster;  // heads of a CTA; cluster divides 8 NT, so cluster * own <= 8 NT rows
   W w;
   w.lane = lane;
   w.ring = smem_u32(smem) + warp * kDecRingBytes;
-  w.run(A, b, h, head0, heads, rank * kUnit + warp * W::TT, cluster * kUnit, seq_len_of(A, b));
+  w.template run<true>(A, b, h, head0, heads, rank * kUnit + warp * W::TT, cluster * kUnit, seq_len_of(A, b));
   w.store(reinterpret_cast<float*>(smem + warp * kDecRingBytes), s_ml[warp]);
   __syncthreads();
   if (cluster > 1) cluster_started_wait();
