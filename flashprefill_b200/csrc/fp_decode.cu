@@ -39,11 +39,12 @@
 //     score and its V scale its weight, relative to the largest V scale so far (a running reference like the maximum), so
 //     weights stay at most 2^15.
 //
-// Measured (device time; of the measured 6.54 TB/s): 64 x up to 8192 tokens of 32/8 heads, bf16, 1.11 GB, 163 to 171 us (100%
-// and more: reads alone pass a copy's rate); 1 x 131072, 0.54 GB, 85 us (97%); 2 x up to 262144 of 28/4 heads, e4m3, 0.53 GB,
-// 83 to 88 us (92 to 98%), 46% of the issue slots; 33 x up to 16001 of 28/4 heads, e4m3, 0.31 GB, 53 to 57 us (82 to 88%): 3 us from
-// the launch to the first full stream (lengths, table, rows: three loads in turn), 3 us between the first CTA that ends and the
-// last, 4 us for the join.  1 x 500 of 32/8 heads, 2 MB, 4.5 us: the same loads in turn.
+// Measured (device time; of the measured 6.54 TB/s): 64 x up to 8192 tokens of 32/8 heads, bf16, 1.11 GB, 163 to 169 us (100%
+// and more: reads alone pass a copy's rate); 1 x 131072, 0.54 GB, 86 us (95%); 2 x up to 262144 of 28/4 heads, e4m3, 0.53 GB,
+// 83 to 87 us (93 to 97%), 46% of the issue slots; 33 x up to 16001 of 28/4 heads, e4m3, 0.31 GB, 53 to 57 us (82 to 88%): 3 us
+// from the launch to the first full stream (lengths, table, rows: three loads in turn), 3 us between the first CTA that ends
+// and the last, 4 us for the join.  1 x 500 of 32/8 heads, 2 MB, 4.5 us: the launch 0.9, the same loads in turn and the warps'
+// sums 1.8, the cluster's barrier and sums 1.8.
 #include <type_traits>
 
 #include "fp_common.cuh"
@@ -489,8 +490,8 @@ struct DecodeWarp {
 
   // All of this warp's tiles of an item: tokens [tok + i * step, + TT) below min(end, the sequence's length).  The first
   // table entries and q are on their way before the length is needed.  kAhead: the next tile is asked for before, not after,
-  // the wait for this one.  That shortens a warp's chain of tiles (256 x up to 600 tokens 19.6 -> 18.2 us, 1 x 8192 11.6 -> 10.6) but puts
-  // more in flight than long streams bear (64 x up to 8192, bf16: 169 -> 176 us).
+  // the wait for this one.  That shortens a warp's chain of tiles (256 x up to 600 tokens 19.6 -> 18.3 us, 1 x 8192 11.8 ->
+  // 10.6) but puts more in flight than long streams bear (64 x up to 8192, bf16: 168 -> 174 us).
   template <bool kAhead>
   __device__ __forceinline__ void run(const DecodeArgs& A, int b, int h, int head0, int heads, int tok, int step, int end) {
     const int* table = A.page_table + b * A.table_stride;
