@@ -216,6 +216,8 @@ class TPLlamaPrefill:
         Tokens after the first chunk attend to the cached prefix, read back, and to their own keys."""
         from .paged_cache import kv_cache_read, kv_cache_write
         cfg = self.cfg
+        if not 0 <= seq < len(cache.lens):
+            raise ValueError(f"sequence {seq} of the cache's {len(cache.lens)}")
         S, D, n = tokens.shape[0], cfg.head_dim, cache.lens[seq]
         if S < 1 or n + S > cache.max_len:
             raise ValueError(f"{S} tokens after {n} do not fit the cache's {cache.max_len}")

@@ -20,6 +20,18 @@ def test_cache_slots_follow_the_page_table():
     assert got.tolist() == [3 * 16 + 1, 1, 5 * 16 + 15]
 
 
+def test_prefill_refuses_sequences_that_are_not_there():
+    m = TPLlamaPrefill(LlamaConfig(layers=1, hidden=128, q_heads=1, kv_heads=1, ffn=128, vocab=16), device="cpu", dtype=torch.float32)
+    cache = m.new_cache(2, 32, page_size=16, dtype=BF16)
+    for seq in (-1, 2):
+        with pytest.raises(ValueError, match="sequence"):
+            m.prefill(torch.zeros(3, dtype=torch.int64), cache, seq)
+    with pytest.raises(ValueError, match="fit"):
+        m.prefill(torch.zeros(33, dtype=torch.int64), cache, 1)
+    with pytest.raises(ValueError, match="fit"):
+        m.prefill(torch.zeros(0, dtype=torch.int64), cache, 1)
+
+
 def test_registered_ops_trace_and_mutate():
     from torch._subclasses.fake_tensor import FakeTensorMode
     for name, muts in (("kv_cache_write", ("k_cache", "v_cache", "k_scale", "v_scale")), ("kv_cache_read", ("k", "v")),
