@@ -1,0 +1,54 @@
+"""Paged cache and decode attention where the work is cut: more items than pieces, workspaces with stale contents."""
+import pytest
+import torch
+
+import flashprefill_b200 as fp
+from tests import paged_util as pu
+from tests.test_paged_cache import check_decode, same_bits
+
+E4M3 = torch.float8_e4m3fn
+BF16, FP16 = torch.bfloat16, torch.float16
+
+# A GPU of 148 SMs holds 444 CTAs of items of up to 8 heads and 296 of items of 9 to 16: lens, q heads, kv heads, page size, layout
+MANY_ITEMS = [
+    ([0, 1, 700, 64, 65, 17, 300, 2] * 8, 16, 8, 16, "nhd"),                   # 512 items
+    ([33, 0, 129] * 29 + [5, 1000], 15, 5, 48, "hnd"),                         # 445 items, one more than pieces
+    ([9000] + [0, 3, 0, 70, 1] * 60, 2, 2, 64, "hnd"),                         # 602 items, one of them in many pieces
+    ([0] * 299 + [1], 4, 2, 16, "nhd"),                                        # 600 items that hold one token
+    ([257, 0, 31, 16, 1] * 30, 24, 2, 16, "hnd"),                              # 300 items of 12 heads
+    ([5000, 0] + [40, 200, 0] * 99, 16, 1, 5, "nhd"),                          # 299 items of 16 heads
+    ([100, 7, 0, 900] * 38, 20, 1, 32, "nhd"),                                 # 304 items: 20 heads in two groups
+    ([0, 1], 32, 8, 16, "hnd"),                                                # fewer units than CTAs: most leave early
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("case", range(len(MANY_ITEMS)))
+def test_more_items_than_pieces(case, quant, dtype):
+    """Items that no piece begins alone, pieces that span several whole items and two cut ones, lengths of zero among them; in
+    workspaces of zeros, of ones and of an earlier call's sums."""
+    lens, hq, hk, ps, layout = MANY_ITEMS[case]
+    cd = E4M3 if quant else dtype
+    f = pu.fill_sequences(lens, hq, hk, dtype, cd, ps, layout, seed=30 + case, room=70000)
+    n = fp.paged_decode_workspace_bytes(len(lens), hq, hk, cd, f["page_table"].shape[1], ps)
+    assert n > 0  # in pieces, not clusters
+    cache = (f["k"], f["v"])
+    back = torch.arange(len(lens) - 1, -1, -1, device="cuda")
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    first = None
+    for fill in (0, 255, None):
+        if fill is not None:
+            ws.fill_(fill)
+        else:  # the sums and descriptors of other lengths
+            fp.paged_decode(f["q"], *cache, f["page_table"][back], f["lens"][back], torch.empty_like(f["q"]), None, f["k_scale"],
+                            f["v_scale"], workspace=ws)
+        out = torch.full_like(f["q"], float("nan"))
+        lse = torch.full((len(lens), hq), float("nan"), device="cuda")
+        fp.paged_decode(f["q"], *cache, f["page_table"], f["lens"], out, lse, f["k_scale"], f["v_scale"], workspace=ws)
+        fp.check_paged_error()
+        if first is None:
+            first = out, lse
+            check_decode(f, out, lse, dtype, cd)
+        assert same_bits(out, first[0]) and same_bits(lse, first[1])
