@@ -202,6 +202,8 @@ int fpb_kv_cache_write(const void* k, const void* v, int dtype, int tokens, int 
   FPB_TRY(check_strides(k_strides, 2, "k"));
   FPB_TRY(check_strides(v_strides, 2, "v"));
   FPB_CHECK_ARG(slots != nullptr && reinterpret_cast<uintptr_t>(slots) % slot_bytes == 0, "slots must be an aligned pointer");
+  FPB_CHECK_ARG(k_cache != v_cache, "k_cache and v_cache must not be the same memory");
+  FPB_CHECK_ARG(k_scale == nullptr || k_scale != v_scale, "k_scale and v_scale must not be the same memory");
   A.k = static_cast<const uint8_t*>(k);
   A.v = static_cast<const uint8_t*>(v);
   FPB_TRY(make_pitch(&A.kp, 0, 2 * k_strides[0], 2 * k_strides[1], 16, "k"));
@@ -235,6 +237,7 @@ int fpb_kv_cache_read(const void* k_cache, const void* v_cache, int cache_dtype,
   FPB_TRY(check_ptr(v, "v"));
   FPB_TRY(check_strides(k_strides, 3, "k"));
   FPB_TRY(check_strides(v_strides, 3, "v"));
+  FPB_CHECK_ARG(k != v, "k and v must not be the same memory");
   A.page_table = page_table;
   A.table_stride = table_stride;
   A.max_pages = max_pages;

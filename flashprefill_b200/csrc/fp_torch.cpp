@@ -171,6 +171,7 @@ void write_(PyObject* const* a) {
   REFUSE(v.scalar_type() != k.scalar_type(), Type, "k and v must share one dtype");
   const Cache c = cache_args(a[2], a[3], a[5], a[6], k, device, k.size(1), true);
   REFUSE(c.k->data_ptr() == c.v->data_ptr(), Value, "k_cache and v_cache must not be the same memory");
+  REFUSE(c.k_scale && c.k_scale == c.v_scale, Value, "k_scale and v_scale must not be the same memory");
   const at::Tensor& s = tensor(a[4], "slots", 1, &device);
   REFUSE(s.scalar_type() != at::kLong && s.scalar_type() != at::kInt, Type, "slots must be int64 or int32, got ", s.scalar_type());
   REFUSE(s.size(0) != k.size(0), Value, "slots must have one entry for each of the ", k.size(0), " rows, got ", s.size(0));

@@ -54,7 +54,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     An e4m3 cache gets ``scale = max(max|x|, 2**-100) / 448`` and codes ``x / scale`` for each row; a row with an infinity or
     a NaN reads back as NaN.  k and v may have any strides (e.g. columns of a fused projection; copied only where rows are not
     16-byte aligned).  The slots of one call must differ from one another (FLASHPREFILL_B200_CHECK=1 checks that); where two
-    rows name one slot, its contents are not defined.  k_cache and v_cache must be different memory."""
+    rows name one slot, its contents are not defined.  k_cache and v_cache must be different memory, as must the scales."""
     (_lib._ext or _lib.ext()).kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
     if _ops.CHECK:
         _ops.finish_paged(k.device, slots)

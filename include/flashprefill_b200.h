@@ -232,7 +232,8 @@ FPB_API int fpb_read_device_error(const void* workspace, uint32_t* flags, void* 
 
 /* Rows k, v (tokens, hk, 128), strides {token, head}, into the cache slots slots[t] = page * page_size + offset (int32 or
  * int64: slot_bytes 4 or 8).  A negative slot skips its row (padding).  Slots must differ from one another; where two rows
- * name one slot, what it holds is not defined.  For FPB_E4M3 each row's scale is max(max|x|, 2^-100) / 448. */
+ * name one slot, what it holds is not defined.  k_cache and v_cache are different memory, as are k_scale and v_scale.  For
+ * FPB_E4M3 each row's scale is max(max|x|, 2^-100) / 448. */
 FPB_API int fpb_kv_cache_write(const void* k, const void* v, int dtype, int tokens, int hk, int head_dim,
                                const int64_t* k_strides, const int64_t* v_strides, void* k_cache, void* v_cache,
                                int cache_dtype, int num_pages, int page_size, const int64_t* cache_strides,

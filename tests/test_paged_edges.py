@@ -1,8 +1,11 @@
 """Paged cache and decode attention where the work is cut: more items than pieces, workspaces with stale contents."""
+import os
+
 import pytest
 import torch
 
 import flashprefill_b200 as fp
+from flashprefill_b200 import _lib
 from tests import paged_util as pu
 from tests.test_paged_cache import check_decode, same_bits
 
@@ -52,3 +55,34 @@ def test_more_items_than_pieces(case, quant, dtype):
             first = out, lse
             check_decode(f, out, lse, dtype, cd)
         assert same_bits(out, first[0]) and same_bits(lse, first[1])
+
+
+# ------------------------------------------------------------------ memory that two tensors of one call share
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_lib.LIB_PATH):
+        from flashprefill_b200 import build
+        build.build()
+    return _lib.load()
+
+
+def test_c_entries_refuse_one_memory_for_keys_and_values(lib):
+    i = _lib.i64arr
+    def write(kc, vc, cd, ks, vs):
+        ss = i([32, 1, 16]) if cd else None
+        return lib.fpb_kv_cache_write(256, 512, 0, 4, 2, 128, i([256, 128]), i([256, 128]), kc, vc, cd, 8, 16, i([4096, 128, 2048]), ks,
+                                      vs, ss, 1024, 8, None)
+    assert write(4096, 4096, _lib.FPB_BF16, None, None) == _lib.FPB_EINVAL and b"k_cache and v_cache" in lib.fpb_last_error()
+    assert write(4096, 8192, _lib.FPB_E4M3, 64, 64) == _lib.FPB_EINVAL and b"k_scale and v_scale" in lib.fpb_last_error()
+    s = i([40 * 256, 256, 128])
+    assert lib.fpb_kv_cache_read(4096, 8192, 0, 8, 16, 2, 128, i([4096, 128, 2048]), None, None, None, 256, 4, 4, 512, 2, 1024, 1024, 0,
+                                 40, s, s, None) == _lib.FPB_EINVAL and b"k and v must not" in lib.fpb_last_error()
+
+
+@pytest.mark.gpu
+def test_write_refuses_one_scale_tensor_for_keys_and_values():
+    """Keys would be read back with the values' scales."""
+    c = fp.kv_cache_alloc(2, 16, 2, E4M3)
+    rows = torch.ones(3, 2, 128, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="k_scale and v_scale must not be the same memory"):
+        fp.kv_cache_write(rows, rows, c.k, c.v, torch.arange(3, device="cuda"), c.k_scale, c.k_scale)
