@@ -149,7 +149,7 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY
 
 // Tokens of sequence b; a length outside [0, room] is reported and counts as 0.
 __device__ __forceinline__ int seq_len_of(const DecodeArgs& A, int b) {
-  const int len = __ldg(A.seq_lens + b);
+  const int len = A.seq_lens[b];
   if (len < 0 || len > (int64_t)A.max_pages * A.C.page_size) {
     raise_error(&g_paged_err, kErrBadLength);
     return 0;
@@ -188,10 +188,10 @@ struct DecodeWarp {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if constexpr (!kE4m3) {
-          qf[n][k][0] = ok ? __ldg(reinterpret_cast<const uint32_t*>(row + 32 * k + 4 * t)) : 0u;
-          qf[n][k][1] = ok ? __ldg(reinterpret_cast<const uint32_t*>(row + 32 * k + 4 * t + 16)) : 0u;
+          qf[n][k][0] = ok ? *reinterpret_cast<const uint32_t*>(row + 32 * k + 4 * t) : 0u;
+          qf[n][k][1] = ok ? *reinterpret_cast<const uint32_t*>(row + 32 * k + 4 * t + 16) : 0u;
         } else {
-          const uint2 x = ok ? __ldg(reinterpret_cast<const uint2*>(row + 32 * k + 8 * t)) : make_uint2(0u, 0u);
+          const uint2 x = ok ? *reinterpret_cast<const uint2*>(row + 32 * k + 8 * t) : make_uint2(0u, 0u);
           qf[n][k][0] = x.x;
           qf[n][k][1] = x.y;
         }
@@ -246,7 +246,7 @@ struct DecodeWarp {
 #pragma unroll
     for (int j = 0; j < MTILES; ++j) {
       const int p = A.C.page_of(tok + 16 * j);
-      page[j] = p < A.max_pages ? __ldg(table + p) : -1;
+      page[j] = p < A.max_pages ? table[p] : -1;
     }
   }
 
@@ -302,7 +302,7 @@ struct DecodeWarp {
     int64_t off = -1;
     uint64_t so = 0;
     if (my < end) {
-      const int p = A.C.page_of(my), at = my - p * A.C.page_size, pg = __ldg(table + p);
+      const int p = A.C.page_of(my), at = my - p * A.C.page_size, pg = table[p];
       if ((unsigned)pg < (unsigned)A.C.num_pages) {
         off = (int64_t)(A.C.rows.at(pg, at, h) * 16);
         if constexpr (kE4m3) so = A.C.scales.at(pg, at, h);

@@ -15,9 +15,8 @@
 // shrink with its elements (amax over the lanes, the division, the addresses) would bound it with 16 lanes (131072 tokens of
 // 8 heads, bf16 to e4m3: 177 us against 134).  Where a read is large enough to fill the GPU all the same and 4 divides
 // page_size, the lanes take 4 tokens of a head: one table entry and one division for all, and their loads under way together (the same
-// tokens read back: 127 us, 140 token by token).  Rows come through the read-only path: as they are read once, loads that
-// leave the caches first might seem right, but the rows were written just before, and are still in L2 in the calls that
-// matter (4099 tokens of 2 heads to e4m3: 2.5 us, 2.9 so).
+// tokens read back: 127 us, 140 token by token).  As rows are read once, loads that leave the caches first might seem right, but
+// they were written just before, and are still in L2 in the calls that matter (4099 tokens of 2 heads to e4m3: 2.5 us, 2.9 so).
 // Of the measured 6.54 TB/s at 131072 tokens of 8 heads: copying 101%, quantising 94% (58% of the issue slots), reading e4m3 98%.
 #include "fp_common.cuh"
 
@@ -68,7 +67,10 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
 // The kernels of the paged cache are short and follow one another (write, decode, join, the next layer's write ...), so each
 // is launched with programmatic stream serialisation, which prepares its launch while its predecessor still runs, and waits
 // here, before it touches memory, until all that came before it on the stream is complete and visible (1 x 500 tokens
-// decode: 6.2 us a call without, 4.6 with).
+// decode: 6.2 us a call without, 4.6 with).  What it then reads may have been written while it was already launched, so its
+// loads are ordinary ones: the read-only path (__ldg) asks for memory that no one writes for as long as the kernel lives, and
+// the compiler may move such loads, even in front of the wait (without them 131072 tokens to e4m3 take 126.2 us, 125.5 with;
+// 1 x 500 tokens decode 4.4, 4.5 with).
 __device__ __forceinline__ void await_stream() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // (a0, a1) * b, two products in one instruction
@@ -103,8 +105,7 @@ struct KvWriteArgs {
 };
 
 __device__ __forceinline__ int64_t load_slot(const KvWriteArgs& A, unsigned tok) {
-  return A.slots64 ? __ldg(static_cast<const long long*>(A.slots) + tok)
-                   : (int64_t)__ldg(static_cast<const int*>(A.slots) + tok);
+  return A.slots64 ? static_cast<const int64_t*>(A.slots)[tok] : static_cast<const int*>(A.slots)[tok];
 }
 
 // (page, offset) of a slot; false for padding (negative) and for a slot outside the cache, which is reported.
@@ -158,9 +159,9 @@ __global__ void __launch_bounds__(kRowThreads, kE4m3 ? 6 : 8) kv_write_kernel(co
   const uint4* vp = reinterpret_cast<const uint4*>(A.v) + A.vp.at(0, tok, h) + c * kPieces;
   uint4 kx[kPieces], vx[kPieces];
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) kx[i] = __ldg(kp + i);
+  for (int i = 0; i < kPieces; ++i) kx[i] = kp[i];
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) vx[i] = __ldg(vp + i);
+  for (int i = 0; i < kPieces; ++i) vx[i] = vp[i];
   int64_t page;
   int at;
   if (!decode_slot(A.C, slot, page, at)) return;  // the same for all lanes of a row
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvReadArgs A
   constexpr int kLanes = row_lanes(false);
   await_stream();
   const unsigned c = threadIdx.x % kLanes, item = blockIdx.x * block_rows(false) + threadIdx.x / kLanes;
-  const int b = blockIdx.y, len = __ldg(A.seq_lens + b);
+  const int b = blockIdx.y, len = A.seq_lens[b];
   if (len < 0 || len > min((int64_t)A.max_pages * A.C.page_size, (int64_t)A.out_len)) {
     raise_error(&g_paged_err, kErrBadLength);
     return;
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvReadArgs A
   const int group = A.group_of(item), h = item - group * A.hk, s = group * kGroup, n = len - s;
   if (n <= 0) return;
   const int p = A.C.page_of(s), at = s - p * A.C.page_size;
-  const int page = __ldg(A.page_table + b * A.table_stride + p);
+  const int page = A.page_table[b * A.table_stride + p];
   if ((unsigned)page >= (unsigned)A.C.num_pages) {
     raise_error(&g_paged_err, kErrBadPage);
     return;
@@ -235,10 +236,10 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvReadArgs A
 #pragma unroll
     for (int j = 0; j < kGroup; ++j)
       if (j < n) {
-        kx[j] = __ldg(kc + (uint64_t)j * 2 * A.C.rows.tok);
-        vx[j] = __ldg(vc + (uint64_t)j * 2 * A.C.rows.tok);
-        ks[j] = __ldg(A.C.k_scale + soff + (uint64_t)j * A.C.scales.tok);
-        vs[j] = __ldg(A.C.v_scale + soff + (uint64_t)j * A.C.scales.tok);
+        kx[j] = kc[(uint64_t)j * 2 * A.C.rows.tok];
+        vx[j] = vc[(uint64_t)j * 2 * A.C.rows.tok];
+        ks[j] = A.C.k_scale[soff + (uint64_t)j * A.C.scales.tok];
+        vs[j] = A.C.v_scale[soff + (uint64_t)j * A.C.scales.tok];
       }
 #pragma unroll
     for (int j = 0; j < kGroup; ++j)
@@ -253,8 +254,8 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvReadArgs A
 #pragma unroll
     for (int j = 0; j < kGroup; ++j)
       if (j < n) {
-        kx[j] = __ldg(kc + (uint64_t)j * A.C.rows.tok);
-        vx[j] = __ldg(vc + (uint64_t)j * A.C.rows.tok);
+        kx[j] = kc[(uint64_t)j * A.C.rows.tok];
+        vx[j] = vc[(uint64_t)j * A.C.rows.tok];
       }
 #pragma unroll
     for (int j = 0; j < kGroup; ++j)

@@ -86,3 +86,80 @@ def test_write_refuses_one_scale_tensor_for_keys_and_values():
     rows = torch.ones(3, 2, 128, dtype=BF16, device="cuda")
     with pytest.raises(ValueError, match="k_scale and v_scale must not be the same memory"):
         fp.kv_cache_write(rows, rows, c.k, c.v, torch.arange(3, device="cuda"), c.k_scale, c.k_scale)
+
+
+# ------------------------------------------------------------------ launches that are prepared while their predecessors run
+def test_kernels_behind_a_stream_wait_use_no_read_only_loads():
+    """A kernel that is launched while its inputs are still being written must not read them as memory that is constant for its
+    lifetime: __ldg, ld.global.nc and const __restrict__ are free to be moved in front of the wait."""
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    for name in ("fp_paged.cu", "fp_decode.cu"):
+        with open(os.path.join(csrc, name)) as f:
+            code = "\n".join(line.split("//")[0] for line in f)
+        assert "await_stream()" in code
+        for word in ("__ldg", "ld.global.nc", "__restrict__", "__ldca", "ld.const"):
+            assert word not in code, (name, word)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quant", [False, True])
+def test_every_step_sees_what_the_one_before_it_wrote(quant):
+    """Lengths, tables, slots, rows and queries changed on the stream just before each call, a step right behind the other, eagerly
+    and from one captured graph (behind copies and a join of two streams): every step equals the same calls made one by one."""
+    dtype, cd, n = BF16, E4M3 if quant else BF16, 200
+    g = torch.Generator(device="cuda").manual_seed(4)
+    steps = 12
+    rows = torch.randn(steps, 2, n, 2, 128, generator=g, device="cuda").to(dtype)
+    qs = torch.randn(steps, 1, 8, 128, generator=g, device="cuda").to(dtype)
+    orders = torch.stack([torch.randperm(16, generator=g, device="cuda") for _ in range(steps)])
+    tables, lengths = orders.int()[:, None], torch.randint(1, n + 1, (steps, 1), generator=g, device="cuda").int()
+    pos = torch.arange(n, device="cuda")
+
+    def run(apart, stages=None):
+        c = fp.kv_cache_alloc(16, 16, 2, cd)
+        for t in c:
+            if t is not None:
+                t.zero_()
+        table, lens, slots = torch.zeros_like(tables[0]), torch.zeros_like(lengths[0]), torch.zeros(n, dtype=torch.int64, device="cuda")
+        kv, q = torch.zeros_like(rows[0]), torch.zeros_like(qs[0])
+        outs = torch.empty(steps, 1, 8, 128, dtype=dtype, device="cuda")
+        back = torch.empty(steps, 2, 1, n, 2, 128, dtype=dtype, device="cuda").fill_(1.0)
+        wait = torch.cuda.synchronize if apart else lambda: None
+        side = torch.cuda.Stream()
+
+        def all_steps():
+            for i in range(steps):
+                here = torch.cuda.current_stream()
+                side.wait_stream(here)
+                with torch.cuda.stream(side):
+                    table.copy_(tables[i])
+                    lens.copy_(lengths[i])
+                slots.copy_(orders[i][pos // 16] * 16 + pos % 16)
+                kv.copy_(rows[i])
+                q.copy_(qs[i])
+                wait()
+                fp.kv_cache_write(kv[0], kv[1], c.k, c.v, slots, c.k_scale, c.v_scale)
+                wait()
+                here.wait_stream(side)
+                fp.paged_decode(q, c.k, c.v, table, lens, outs[i], None, c.k_scale, c.v_scale)
+                wait()
+                fp.kv_cache_read(c.k, c.v, table, lens, back[i, 0], back[i, 1], c.k_scale, c.v_scale)
+                wait()
+
+        if stages is None:
+            all_steps()
+        else:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                all_steps()
+            for _ in range(stages):
+                outs.zero_()
+                back.fill_(1.0)
+                graph.replay()
+        torch.cuda.synchronize()
+        fp.check_paged_error()
+        return outs, back
+
+    want = run(True)
+    for got in (run(False), run(False), run(False, stages=4)):
+        assert same_bits(got[0], want[0]) and same_bits(got[1], want[1])
