@@ -32,7 +32,9 @@
 //     rescaled, only in tiles where some score exceeds it.
 //   * P is split into two 16-bit parts (the value and its remainder) and multiplied twice: one part alone would leave errors
 //     as large as the output's own rounding.  Only for an e4m3 cache with bf16 output is one part enough: fp16 products, an
-//     eighth of the output's rounding.
+//     eighth of the output's rounding.  Where V may hold infinities (16-bit caches) the first part is rounded towards zero and the
+//     second kept above zero, so that both products of a weight and an infinity have its sign, as the weight's own has: a
+//     remainder of 0 or below 0 would make a NaN of it.
 //   * fp16 products: P is scaled by 2^15 (as the row sum is, so it cancels), which keeps weights down to 2^-29 of the
 //     largest in fp16's normal range.
 //   * e4m3: codes widen to fp16 exactly; q is scaled by a power of two to fit fp16; the token's K scale multiplies its
@@ -143,6 +145,22 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, int rank, float v) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+}
+
+// A pair of weights as two 16-bit parts whose sum they are, to 2^-16 (bf16: truncated, and a remainder of 2^-23 at the least) or
+// 2^-21 and 2^-39 of the largest weight (fp16, which holds weights times 2^15: rounded towards zero, and a remainder of one step
+// at the least).  A weight that is not zero has two parts above zero (fp16: one of 2^-39 or more).
+template <typename T>
+__device__ __forceinline__ void split_weights(float x, float y, uint32_t& first, uint32_t& rest) {
+  if constexpr (DT<T>::is_bf16) {
+    constexpr float kBelowOne = 1.f - 1.1920928955078125e-07f;
+    first = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    rest = DT<T>::pack(fmaf(DT<T>::lo(first), -kBelowOne, x), fmaf(DT<T>::hi(first), -kBelowOne, y));
+  } else {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(first) : "f"(y), "f"(x));
+    const uint32_t r = DT<T>::pack(x - DT<T>::lo(first), y - DT<T>::hi(first));
+    asm("max.f16x2 %0, %1, %2;" : "=r"(rest) : "r"(r), "r"(0x00010001u));
+  }
 }
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
@@ -453,9 +471,15 @@ struct DecodeWarp {
             l[n][j] += p[j];
             if constexpr (kE4m3) p[j] *= vf;
           }
-          const uint32_t hi = DT<MT>::pack(p[0], p[1]);
+          uint32_t hi, lo;
+          if constexpr (!kE4m3) {
+            split_weights<MT>(p[0], p[1], hi, lo);
+          } else {
+            hi = DT<MT>::pack(p[0], p[1]);
+            if constexpr (kSplitP) lo = DT<MT>::pack(p[0] - DT<MT>::lo(hi), p[1] - DT<MT>::hi(hi));
+          }
           pb[n][i][h] = transpose8x8(hi);
-          if constexpr (kSplitP) pl[n][i][h] = transpose8x8(DT<MT>::pack(p[0] - DT<MT>::lo(hi), p[1] - DT<MT>::hi(hi)));
+          if constexpr (kSplitP) pl[n][i][h] = transpose8x8(lo);
         }
       }
 #pragma unroll

@@ -80,8 +80,9 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     token's own row first); GQA with q_heads a multiple of kv_heads.  Writes ``out`` (like q) in place and, if given, ``lse``
     (B, q_heads) float32: log sum exp(sm_scale q.k), with which outputs over parts of a sequence can be joined.
 
-    A sequence of length 0 gives zeros and -inf, as does one whose length is outside [0, P * page_size].  ``sm_scale`` is
-    1/sqrt(128) by default.  ``workspace``: uint8 of at least ``paged_decode_workspace_bytes``, taken from the caching
+    A sequence of length 0 gives zeros and -inf, as does one whose length is outside [0, P * page_size].  Infinite values of a
+    16-bit cache keep to the softmax (any weight makes the channel infinite; a weight that vanishes, below 2^-39 of the largest
+    for float16 and 2^-100 for bfloat16, makes it NaN, as 0 times infinity).  ``sm_scale`` is 1/sqrt(128) by default.  ``workspace``: uint8 of at least ``paged_decode_workspace_bytes``, taken from the caching
     allocator by default; calls that may overlap on the GPU (other streams, graphs replayed side by side) need one each.
     Results do not depend on the order in which the GPU runs its blocks: the same call gives the same bits."""
     (_lib._ext or _lib.ext()).paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale,

@@ -163,3 +163,50 @@ def test_every_step_sees_what_the_one_before_it_wrote(quant):
     want = run(True)
     for got in (run(False), run(False), run(False, stages=4)):
         assert same_bits(got[0], want[0]) and same_bits(got[1], want[1])
+
+
+# ------------------------------------------------------------------ values that are not finite, scales far apart
+def check_rows(f, out, lse, dtype, cache_dtype):
+    """Infinities and NaN where the definition in 64 bits has them, all else within its bounds."""
+    for b, (k, v) in enumerate(f["rows"]):
+        ref, rl, _, _ = pu.attend64(f["q"][b], k, v)
+        finite, _, weight, size = pu.attend64(f["q"][b], k, torch.where(v.isfinite(), v, 0.0))
+        to, tl = pu.decode_bounds(finite, rl, weight, size, k.shape[0], dtype, cache_dtype, f["q"][b], k, torch.where(v.isfinite(), v, 0.0))
+        got, there = out[b].double(), ref.isfinite()
+        assert torch.equal(got[~there].nan_to_num(7.0, 8.0, 9.0), ref[~there].nan_to_num(7.0, 8.0, 9.0)), b
+        err = (got - ref).abs()[there]
+        assert (err <= to[there]).all(), (b, (err / to[there]).max().item())
+        assert ((lse[b].double() - rl).abs() <= tl).all(), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [0, 50000])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_infinite_values_follow_the_softmax(dtype, room):
+    """An infinite value with any weight makes its channel infinite, with its sign (the token of the largest weight, of ordinary
+    ones, a sequence of one token); two of opposite signs make NaN; nothing else changes."""
+    f = pu.fill_sequences([700, 300, 1, 65], 8, 2, dtype, dtype, 16, seed=40, k_gain=0.3, room=room)
+
+    def put(b, at, head, channel, x):
+        f["v"][f["page_table"][b, at // 16].long(), at % 16, head, channel] = x
+        f["rows"][b][1][at, head, channel] = x
+
+    inf = float("inf")
+    k, q = f["rows"][0][0], f["q"][0].double()
+    top = torch.einsum("gd,nd->gn", q[:4], k[:, 0]).argmax(-1).tolist()  # heaviest token of each head of KV head 0
+    for i, at in enumerate(top):
+        put(0, at, 0, i, inf)
+        put(0, at, 0, 40 + i, -inf)
+    for i, at in enumerate(range(0, 700, 33)):
+        put(0, at, 1, i, inf if i % 2 else -inf)
+    put(0, 5, 1, 100, inf)
+    put(0, 690, 1, 100, -inf)
+    put(0, 5, 1, 101, inf)
+    put(0, 690, 1, 101, inf)
+    put(2, 0, 0, 3, inf)
+    put(2, 0, 1, 4, -inf)
+    put(3, 64, 0, 127, inf)
+    out, lse = torch.empty_like(f["q"]), torch.empty(4, 8, device="cuda")
+    fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], out, lse)
+    assert out[0].isinf().any() and out[0, 4:, 100].isnan().all() and out[2, :4, 3].eq(inf).all()
+    check_rows(f, out, lse, dtype, dtype)
