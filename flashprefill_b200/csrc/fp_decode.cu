@@ -38,8 +38,10 @@
 //   * fp16 products: P is scaled by 2^15 (as the row sum is, so it cancels), which keeps weights down to 2^-29 of the
 //     largest in fp16's normal range.
 //   * e4m3: codes widen to fp16 exactly; q is scaled by a power of two to fit fp16; the token's K scale multiplies its
-//     score and its V scale its weight, relative to the largest V scale so far (a running reference like the maximum), so
-//     weights stay at most 2^15.
+//     score and its V scale its weight.  These products must fit fp16, so the running maximum is that of score + log2(V scale)
+//     and they reach 2^15; the sum of the weights goes by the same reference and is brought to [1, 2) when an item ends.
+//     (With weights relative to the largest score and V scales to the largest of any token, a row of small values behind one of
+//     large values lost bits, and all of them from 2^39 on, even where the softmax gave the large ones no weight.)
 //
 // Measured (device time; of the measured 6.54 TB/s): 64 x up to 8192 tokens of 32/8 heads, bf16, 1.11 GB, 163 to 169 us (100%
 // and more: reads alone pass a copy's rate); 1 x 131072, 0.54 GB, 86 us (95%); 2 x up to 262144 of 28/4 heads, e4m3, 0.53 GB,
@@ -186,14 +188,16 @@ struct DecodeWarp {
   static constexpr uint32_t kFull = TT == 32 ? 0xFFFFFFFFu : 0xFFFFu;
   static constexpr bool kSplitP = !(kE4m3 && DT<T>::is_bf16);    // P as two parts
   static constexpr float kShift = DT<MT>::is_bf16 ? 0.f : 15.f;  // log2 of the factor of P and l
+  // V scales as the running maximum takes them: P is kept finite beyond, and the sum of 2^31 weights below.
+  static constexpr float kLeastScale = 8.271806125530277e-25f;   // 2^-80
+  static constexpr float kLargestScale = 1.329227995784916e36f;  // 2^120
 
   uint32_t ring;  // shared address of this warp's ring
   int lane;
   uint32_t qf[NT][8][2];      // q as the B operand
   float qc[NT][2];            // factor of this thread's two columns (heads 2t, 2t + 1)
   float o[NT][8][4];          // out^T: 16 channels x 8 heads a tile
-  float m[NT][2], l[NT][2];   // running maximum and this thread's share of the sum
-  float vref, vinv;           // e4m3: largest V scale so far and its reciprocal
+  float m[NT][2], l[NT][2];   // running maximum (e4m3: of score + log2 of V's scale) and this thread's share of the sum
 
   // q's rows as they are in memory.  An e4m3 row gives a thread elements 4t .. 4t+3 of each 16: they take the places 2t,
   // 2t+1, 2t+8, 2t+9 of the product's inner dimension, in q as in K.
@@ -255,8 +259,6 @@ struct DecodeWarp {
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
     }
-    vref = 1.1754943508222875e-38f;
-    vinv = 1.f / vref;
   }
 
   // Table entries of the tile at `tok` (one for each 16 tokens).  Entries behind the sequence may be read, never used.
@@ -387,11 +389,7 @@ struct DecodeWarp {
           for (int j = 0; j < 4; ++j) s[n][0][j] += s2[n][j];
       }
     }
-    // scores in log2 units; the largest of this thread's rows g, g + 8 (+ 16 i) for its columns 2t + j
-    bool moved = false;
-    float mx[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;
+    // scores in log2 units
 #pragma unroll
     for (int i = 0; i < MTILES; ++i)
 #pragma unroll
@@ -417,25 +415,26 @@ struct DecodeWarp {
             for (int n = 0; n < NT; ++n) s[n][i][2 * h] = s[n][i][2 * h + 1] = -INFINITY;
           }
     }
+    // the largest of this thread's rows g, g + 8 (+ 16 i) for its columns 2t + j
+    float mx[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int i = 0; i < MTILES; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int h = 0; h < 2; ++h) {
+        float lv = 0.f;
+        if constexpr (kE4m3) lv = __log2f(fminf(fmaxf(fabsf(lds(vsd + 4 * (16 * i + 8 * h + g))), kLeastScale), kLargestScale));
 #pragma unroll
-        for (int i = 0; i < MTILES; ++i) mx[n][j] = fmaxf(mx[n][j], fmaxf(s[n][i][j], s[n][i][2 + j]));
-        moved |= mx[n][j] > m[n][j];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float x = kE4m3 ? s[n][i][2 * h + j] + lv : s[n][i][2 * h + j];
+            mx[n][j] = i + h == 0 ? x : fmaxf(mx[n][j], x);
+          }
       }
-    const float vs = kE4m3 ? lds(vsd + 4 * lane) : 0.f;
-    if constexpr (kE4m3) moved |= !(vs <= vref);
+    bool moved = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) moved |= mx[n][0] > m[n][0] || mx[n][1] > m[n][1];
     if (__any_sync(0xffffffffu, moved)) {
-      float vcorr = 1.f;
-      if constexpr (kE4m3) {
-        const float vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vs)));
-        const float vnew = vmax <= vref ? vref : vmax;
-        vcorr = vnew == vref ? 1.f : vref / vnew;
-        vref = vnew;
-        vinv = 1.f / vnew;
-      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float corr[2];
@@ -447,7 +446,7 @@ struct DecodeWarp {
           const float mn = fmaxf(m[n][j], x), f = ex2_approx(m[n][j] - finite_or_zero(mn));
           m[n][j] = mn;
           l[n][j] *= f;
-          corr[j] = f * vcorr;
+          corr[j] = f;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -460,8 +459,8 @@ struct DecodeWarp {
     for (int i = 0; i < MTILES; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float vf = 1.f;
-        if constexpr (kE4m3) vf = lds(vsd + 4 * (16 * i + 8 * h + g)) * vinv;
+        float vs = 1.f;
+        if constexpr (kE4m3) vs = lds(vsd + 4 * (16 * i + 8 * h + g));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float p[2];
@@ -469,7 +468,7 @@ struct DecodeWarp {
           for (int j = 0; j < 2; ++j) {
             p[j] = ex2_approx(s[n][i][2 * h + j] - (finite_or_zero(m[n][j]) - kShift));
             l[n][j] += p[j];
-            if constexpr (kE4m3) p[j] *= vf;
+            if constexpr (kE4m3) p[j] *= vs;
           }
           uint32_t hi, lo;
           if constexpr (!kE4m3) {
@@ -579,10 +578,12 @@ struct DecodeWarp {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
         const int h = n * 8 + 2 * t + j;
-        if (g == 0) sml[h] = make_float2(m[n][j] - kShift, x);
+        int e = 0;
+        if constexpr (kE4m3) e = max(-120, min((int)(__float_as_uint(x) >> 23) - 127, 120));
+        const float f = exp2i(-e);
+        if (g == 0) sml[h] = make_float2(m[n][j] - kShift + (float)e, x * f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float f = kE4m3 ? vref : 1.f;
           const int d0 = 16 * i + (kE4m3 ? 2 * g : g), d1 = 16 * i + (kE4m3 ? 2 * g + 1 : g + 8);
           so[h * 132 + d0] = o[n][i][j] * f;
           so[h * 132 + d1] = o[n][i][2 + j] * f;

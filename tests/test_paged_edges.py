@@ -210,3 +210,64 @@ def test_infinite_values_follow_the_softmax(dtype, room):
     fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], out, lse)
     assert out[0].isinf().any() and out[0, 4:, 100].isnan().all() and out[2, :4, 3].eq(inf).all()
     check_rows(f, out, lse, dtype, dtype)
+
+
+def weighted_bounds(q, k, v, dtype, cache_dtype):
+    """attend64's results with bounds whose fp16 steps, 2^-40 of each, are those of the largest product of a head's weight and a row's
+    largest value."""
+    ref, lse, weight, size = pu.attend64(q, k, v)
+    n, hk = k.shape[0], k.shape[1]
+    to, tl = pu.decode_bounds(ref, lse, weight, size, n, dtype, cache_dtype, q, k, torch.zeros_like(v))
+    s = torch.einsum("hgd,nhd->hgn", q.double().view(hk, -1, 128), k) * 128 ** -0.5
+    largest = (torch.softmax(s, -1) * v.abs().amax(-1).t()[:, None]).amax(-1).reshape(-1, 1)
+    return ref, lse, to + n * 2.0 ** -40 * largest, tl
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [0, 70000])
+@pytest.mark.parametrize("heads", [4, 12])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_value_scales_far_apart(dtype, heads, room):
+    """A quantised row keeps its bits whatever the scales of the others: rows of values up to 2^90 times as large that the softmax
+    gives no weight (in front, behind and between), scales that rise and fall through the sequence, and weights that make up
+    for the scales."""
+    f = pu.fill_sequences([300, 300, 513, 600, 40], heads, 1, dtype, E4M3, 16, seed=50, k_gain=0.2, room=room)
+    f["q"] = f["q"].abs() + 0.1  # so that a key of like values has a score of its sign for every head
+
+    def at(b, i):
+        i = torch.as_tensor(i, device="cuda")
+        return f["page_table"][b].long()[i // 16], i % 16
+
+    def gain(b, i, x):
+        p = at(b, i)
+        f["v_scale"][p[0], p[1]] *= x[:, None]
+        f["rows"][b][1][i] *= x.double()[:, None, None]
+
+    def no_weight(b, i):
+        p = at(b, i)
+        f["k"].view(torch.uint8)[p[0], p[1]] = torch.tensor(-448.0).to(E4M3).view(torch.uint8).item()
+        f["k_scale"][p[0], p[1]] = 1.0  # score below -448 * 0.1 * sqrt(128) = -500
+        f["rows"][b][0][i] = -448.0
+
+    for b, i in ((0, [0, 1, 40]), (1, [299]), (2, list(range(31, 513, 64)))):
+        no_weight(b, i)
+        gain(b, i, torch.full((len(i),), 2.0 ** (90 if b else 45), device="cuda"))
+    n = 600
+    i = torch.arange(n, device="cuda")
+    gain(3, i, torch.exp2(-20.0 * torch.sin(i / 25.0).abs()))
+    i = torch.arange(40, device="cuda")
+    gain(4, i, torch.exp2(-2.0 * i))
+    # a key of like values c has the score c * sum(q) / sqrt(128): about 1.5 nats a token, more than the 1.4 that its values lose
+    p = at(4, i)
+    c = 1.5 / (f["q"][4].float().sum(-1).min() * 128 ** -0.5)
+    f["k"].view(torch.uint8)[p[0], p[1]] = torch.tensor(1.0).to(E4M3).view(torch.uint8).item()
+    f["k_scale"][p[0], p[1]] = (c * i)[:, None]
+    f["rows"][4][0][i] = (c * i).float().double()[:, None, None].expand(40, 1, 128)
+    out, lse = torch.empty_like(f["q"]), torch.empty(5, heads, device="cuda")
+    fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], out, lse, f["k_scale"], f["v_scale"])
+    fp.check_paged_error()
+    for b, (k, v) in enumerate(f["rows"]):
+        ref, rl, to, tl = weighted_bounds(f["q"][b], k, v, dtype, E4M3)
+        err = (out[b].double() - ref).abs()
+        assert (err <= to).all(), (b, (err / to).max().item(), ref.abs().max().item())
+        assert ((lse[b].double() - rl).abs() <= tl).all(), b
