@@ -37,7 +37,7 @@
 //     remainder of 0 or below 0 would make a NaN of it.
 //   * fp16 products: P is scaled by 2^15 (as the row sum is, so it cancels), which keeps weights down to 2^-29 of the
 //     largest in fp16's normal range.
-//   * e4m3: codes widen to fp16 exactly; q is scaled by a power of two to fit fp16; the token's K scale multiplies its
+//   * e4m3: codes widen to fp16 exactly; q is scaled by a power of two to fill fp16's range; the token's K scale multiplies its
 //     score and its V scale its weight.  These products must fit fp16, so the running maximum is that of score + log2(V scale)
 //     and they reach 2^15; the sum of the weights goes by the same reference and is brought to [1, 2) when an item ends.
 //     (With weights relative to the largest score and V scales to the largest of any token, a row of small values behind one of
@@ -233,9 +233,9 @@ struct DecodeWarp {
         mx = max(mx & 0xFFFFu, mx >> 16);
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // power of two that brings the row's largest magnitude to [1, 2); inf and NaN pass as they are
-        int e = (int)(mx >> 7) - 127;
-        e = max(-120, min(e, 120));
+        // power of two that brings the row's largest magnitude to [2^14, 2^15), which leaves elements 2^28 times smaller in
+        // fp16's normal range; inf and NaN pass as they are
+        const int e = max(-120, (int)(mx >> 7) - 127 - 14);
         const float down = exp2i(-e);
         f = exp2i(e);
 #pragma unroll

@@ -271,3 +271,23 @@ def test_value_scales_far_apart(dtype, heads, room):
         err = (out[b].double() - ref).abs()
         assert (err <= to).all(), (b, (err / to).max().item(), ref.abs().max().item())
         assert ((lse[b].double() - rl).abs() <= tl).all(), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("small", [2.0 ** -13, 2.0 ** -20, 2.0 ** -26])
+def test_small_elements_of_a_query_beside_large_ones(small):
+    """bfloat16 queries over a quantised cache, multiplied in fp16: elements far below their row's largest keep their bits where the
+    keys do not meet the large one.  An element is off by 2^-39 of the largest at the most."""
+    f = pu.fill_sequences([90, 700], 6, 2, BF16, E4M3, 16, seed=60)
+    f["q"] *= small
+    f["q"][:, :, 17] = 1.0
+    f["k"].view(torch.uint8)[..., 17] = 0
+    for k, _ in f["rows"]:
+        k[..., 17] = 0.0
+    scale = 128 ** -0.5 / small
+    out, lse = torch.empty_like(f["q"]), torch.empty(2, 6, device="cuda")
+    fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], out, lse, f["k_scale"], f["v_scale"], sm_scale=scale)
+    for b, (k, v) in enumerate(f["rows"]):
+        ref, rl, weight, size = pu.attend64(f["q"][b], k, v, scale)
+        to, tl = pu.decode_bounds(ref, rl, weight, size, k.shape[0], BF16, E4M3, f["q"][b] * 2.0 ** -15, k, v, scale)
+        assert ((out[b].double() - ref).abs() <= to).all() and ((lse[b].double() - rl).abs() <= tl).all(), b
