@@ -31,10 +31,11 @@
 //   * Scores, maxima, sums and outputs stay in fp32 registers.  The running maximum is reduced over the warp, and sums are
 //     rescaled, only in tiles where some score exceeds it.
 //   * P is split into two 16-bit parts (the value and its remainder) and multiplied twice: one part alone would leave errors
-//     as large as the output's own rounding.  Only for an e4m3 cache with bf16 output is one part enough: fp16 products, an
-//     eighth of the output's rounding.  Where V may hold infinities (16-bit caches) the first part is rounded towards zero and the
-//     second kept above zero, so that both products of a weight and an infinity have its sign, as the weight's own has: a
-//     remainder of 0 or below 0 would make a NaN of it.
+//     as large as the output's own rounding, or for fp16 products and bf16 output an eighth of it.  (One part there: 33 x 16K
+//     e4m3 52.9 us, 53.5 with two; 2 x 256K 82.5 and 82.4; 12 heads a KV head 40.6 and 45.)
+//     Where V may hold infinities (16-bit caches) the first part is rounded towards zero and the second kept above zero, so
+//     that both products of a weight and an infinity have its sign, as the weight's own has: a remainder of 0 or below 0 would
+//     make a NaN of it.
 //   * fp16 products: P is scaled by 2^15 (as the row sum is, so it cancels), which keeps weights down to 2^-29 of the
 //     largest in fp16's normal range.
 //   * e4m3: codes widen to fp16 exactly; q is scaled by a power of two to fill fp16's range; the token's K scale multiplies its
@@ -186,7 +187,6 @@ struct DecodeWarp {
   static constexpr int kRowBytes = kDecTileBytes / TT;
   static constexpr int kChunks = kRowBytes / 16;  // 16-byte pieces of a row
   static constexpr uint32_t kFull = TT == 32 ? 0xFFFFFFFFu : 0xFFFFu;
-  static constexpr bool kSplitP = !(kE4m3 && DT<T>::is_bf16);    // P as two parts
   static constexpr float kShift = DT<MT>::is_bf16 ? 0.f : 15.f;  // log2 of the factor of P and l
   // V scales as the running maximum takes them: P is kept finite beyond, and the sum of 2^31 weights below.
   static constexpr float kLeastScale = 8.271806125530277e-25f;   // 2^-80
@@ -475,10 +475,10 @@ struct DecodeWarp {
             split_weights<MT>(p[0], p[1], hi, lo);
           } else {
             hi = DT<MT>::pack(p[0], p[1]);
-            if constexpr (kSplitP) lo = DT<MT>::pack(p[0] - DT<MT>::lo(hi), p[1] - DT<MT>::hi(hi));
+            lo = DT<MT>::pack(p[0] - DT<MT>::lo(hi), p[1] - DT<MT>::hi(hi));
           }
           pb[n][i][h] = transpose8x8(hi);
-          if constexpr (kSplitP) pl[n][i][h] = transpose8x8(lo);
+          pl[n][i][h] = transpose8x8(lo);
         }
       }
 #pragma unroll
@@ -490,7 +490,7 @@ struct DecodeWarp {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           mma16816<MT>(o[n][i], a[0], a[1], a[2], a[3], pb[n][0][0], pb[n][0][1]);
-          if constexpr (kSplitP) mma16816<MT>(o[n][i], a[0], a[1], a[2], a[3], pl[n][0][0], pl[n][0][1]);
+          mma16816<MT>(o[n][i], a[0], a[1], a[2], a[3], pl[n][0][0], pl[n][0][1]);
         }
       } else {
         // transposed pairs of codes: {token 2t: channels 2g, 2g+1; token 2t+1: channels 2g, 2g+1}; channel 2g becomes
@@ -504,7 +504,7 @@ struct DecodeWarp {
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma16816<MT>(o[n][i], a0, a1, a2, a3, pb[n][k][0], pb[n][k][1]);
-            if constexpr (kSplitP) mma16816<MT>(o[n][i], a0, a1, a2, a3, pl[n][k][0], pl[n][k][1]);
+            mma16816<MT>(o[n][i], a0, a1, a2, a3, pl[n][k][0], pl[n][k][1]);
           }
         }
       }

@@ -291,3 +291,25 @@ def test_small_elements_of_a_query_beside_large_ones(small):
         ref, rl, weight, size = pu.attend64(f["q"][b], k, v, scale)
         to, tl = pu.decode_bounds(ref, rl, weight, size, k.shape[0], BF16, E4M3, f["q"][b] * 2.0 ** -15, k, v, scale)
         assert ((out[b].double() - ref).abs() <= to).all() and ((lse[b].double() - rl).abs() <= tl).all(), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [0, 70000])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_weights_keep_more_bits_than_their_products_type(dtype, room):
+    """Rows of 1 and of -(1 + 2^-13) in equal parts: what is left of their sum, 2^-14, is below one rounding of a weight to fp16."""
+    n = 64
+    f = pu.fill_sequences([n], 4, 1, dtype, E4M3, 16, seed=61, room=room)
+    page, at = f["page_table"][0].long()[torch.arange(n, device="cuda") // 16], torch.arange(n, device="cuda") % 16
+    f["k"].view(torch.uint8)[page, at] = 0
+    sign = torch.where(torch.arange(n, device="cuda") % 2 == 0, 1.0, -1.0)
+    scale = torch.where(sign > 0, 1.0, 1.0 + 2.0 ** -13)
+    f["v"].view(torch.uint8)[page, at] = sign[:, None, None].expand(n, 1, 128).to(E4M3).view(torch.uint8)
+    f["v_scale"][page, at] = scale[:, None]
+    k, v = torch.zeros(n, 1, 128, dtype=torch.float64, device="cuda"), (sign * scale).double()[:, None, None].expand(n, 1, 128)
+    out = torch.empty_like(f["q"])
+    fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], out, None, f["k_scale"], f["v_scale"])
+    ref, _, weight, size = pu.attend64(f["q"][0], k, v)
+    # weights as two fp16 parts, 2^-21; their sum in fp32, n 2^-24; exp2 and the scale's product, 2^-21
+    bound = (2.0 ** -21 + (n + 16) * 2.0 ** -24 + 2.0 ** -21) * weight + pu.half_step(dtype) * ref.abs()
+    assert (ref.abs() > 4 * bound).all() and ((out[0].double() - ref).abs() <= bound).all()
