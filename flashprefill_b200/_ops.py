@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 
 import torch
 
@@ -333,15 +334,23 @@ def check_paged_error(device=None) -> None:
     _lib.check(rc)
 
 
-def finish_paged(device, slots=None) -> None:
-    """After a paged-cache call with FLASHPREFILL_B200_CHECK set: raise what it met on the device."""
-    if torch.cuda.is_current_stream_capturing():
-        return
-    if slots is not None:
-        used = slots[slots >= 0]
-        if used.unique().numel() != used.numel():
-            raise ValueError("two rows name one slot")
-    check_paged_error(device)
+_paged_check = threading.Lock()
+
+
+def checked_paged(call, args, slots=None) -> None:
+    """A paged-cache call with FLASHPREFILL_B200_CHECK set: raise what it met on the device (nothing where it is captured).
+    The device's error word is one for all callers, so checked calls run one at a time, each to its end."""
+    with _paged_check:
+        call(*args)
+        device = args[0].device
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                return
+        if slots is not None:
+            used = slots[slots >= 0]
+            if used.unique().numel() != used.numel():
+                raise ValueError("two rows name one slot")
+        check_paged_error(device)
 
 
 def paged_decode_workspace_bytes(batch, q_heads, kv_heads, cache_dtype, max_pages, page_size) -> int:

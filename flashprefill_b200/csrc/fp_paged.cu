@@ -266,6 +266,8 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvReadArgs A
   }
 }
 
-__global__ void paged_clear_err_kernel(uint32_t bits) { atomicAnd(&g_paged_err, ~bits); }
+// Takes the error bits and clears them in one step: a bit that another stream's kernel sets afterwards stays for the next read.
+__device__ uint32_t g_paged_taken;
+__global__ void paged_take_err_kernel() { g_paged_taken = atomicExch(&g_paged_err, 0u); }
 
 }  // namespace fpb

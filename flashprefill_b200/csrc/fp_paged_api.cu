@@ -327,15 +327,15 @@ int fpb_paged_decode(const void* q, int dtype, int batch, int hq, int hk, int he
 int fpb_paged_read_device_error(uint32_t* flags, void* stream) {
   FPB_CHECK_ARG(flags != nullptr, "flags is NULL");
   auto st = static_cast<cudaStream_t>(stream);
+  static std::mutex one_at_a_time;  // g_paged_taken holds one reader's bits
+  const std::lock_guard<std::mutex> lock(one_at_a_time);
   uint32_t h = 0;
-  FPB_CUDA(cudaMemcpyFromSymbolAsync(&h, g_paged_err, sizeof(h), 0, cudaMemcpyDeviceToHost, st));
+  paged_take_err_kernel<<<1, 1, 0, st>>>();
+  FPB_CUDA(cudaGetLastError());
+  FPB_CUDA(cudaMemcpyFromSymbolAsync(&h, g_paged_taken, sizeof(h), 0, cudaMemcpyDeviceToHost, st));
   FPB_CUDA(cudaStreamSynchronize(st));
   *flags = h;
-  if (h == 0) return FPB_OK;
-  paged_clear_err_kernel<<<1, 1, 0, st>>>(h);
-  FPB_CUDA(cudaGetLastError());
-  FPB_CUDA(cudaStreamSynchronize(st));
-  return fail(FPB_EDEVICE, "device error bits 0x%x", h);
+  return h == 0 ? FPB_OK : fail(FPB_EDEVICE, "device error bits 0x%x", h);
 }
 
 }  // extern "C"

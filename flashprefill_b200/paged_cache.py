@@ -12,8 +12,9 @@ its slot is ``page * page_size + offset``.
 
 All calls are asynchronous on the current stream, allocate nothing but a decode call's workspace, never synchronise, and
 can be captured in a CUDA graph.  Slots, pages and lengths are checked on the device: one that points outside its tensors is skipped and
-reported by ``check_paged_error`` (with FLASHPREFILL_B200_CHECK=1 by the call itself).  Shapes, types and strides that are
-not supported raise ValueError or TypeError.
+reported by ``check_paged_error``, which waits for the current stream and clears what all calls on the device have met (with
+FLASHPREFILL_B200_CHECK=1 by the call itself, which then runs alone; a captured call reports to whoever checks after its replay).
+Shapes, types and strides that are not supported raise ValueError or TypeError.
 """
 from __future__ import annotations
 
@@ -55,9 +56,10 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     a NaN reads back as NaN.  k and v may have any strides (e.g. columns of a fused projection; copied only where rows are not
     16-byte aligned).  The slots of one call must differ from one another (FLASHPREFILL_B200_CHECK=1 checks that); where two
     rows name one slot, its contents are not defined.  k_cache and v_cache must be different memory, as must the scales."""
-    (_lib._ext or _lib.ext()).kv_cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
+    write = (_lib._ext or _lib.ext()).kv_cache_write
     if _ops.CHECK:
-        _ops.finish_paged(k.device, slots)
+        return _ops.checked_paged(write, (k, v, k_cache, v_cache, slots, k_scale, v_scale), slots)
+    write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
 
 
 def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -67,9 +69,10 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torc
     ``flash_prefill`` takes for a cached prefix, dequantising an e4m3 cache to their 16-bit type.  Rows from ``seq_lens[b]`` on
     are left as they were, as is all of a sequence whose length is outside [0, S].  page_table (B, P) and seq_lens (B,) are
     int32."""
-    (_lib._ext or _lib.ext()).kv_cache_read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale)
+    read = (_lib._ext or _lib.ext()).kv_cache_read
     if _ops.CHECK:
-        _ops.finish_paged(k.device)
+        return _ops.checked_paged(read, (k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale))
+    read(k_cache, v_cache, page_table, seq_lens, k, v, k_scale, v_scale)
 
 
 def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -85,7 +88,7 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     for float16 and 2^-100 for bfloat16, makes it NaN, as 0 times infinity).  ``sm_scale`` is 1/sqrt(128) by default.  ``workspace``: uint8 of at least ``paged_decode_workspace_bytes``, taken from the caching
     allocator by default; calls that may overlap on the GPU (other streams, graphs replayed side by side) need one each.
     Results do not depend on the order in which the GPU runs its blocks: the same call gives the same bits."""
-    (_lib._ext or _lib.ext()).paged_decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale,
-                                           workspace)
+    decode = (_lib._ext or _lib.ext()).paged_decode
     if _ops.CHECK:
-        _ops.finish_paged(q.device)
+        return _ops.checked_paged(decode, (q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale, workspace))
+    decode(q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale, workspace)

@@ -313,3 +313,87 @@ def test_weights_keep_more_bits_than_their_products_type(dtype, room):
     # weights as two fp16 parts, 2^-21; their sum in fp32, n 2^-24; exp2 and the scale's product, 2^-21
     bound = (2.0 ** -21 + (n + 16) * 2.0 ** -24 + 2.0 ** -21) * weight + pu.half_step(dtype) * ref.abs()
     assert (ref.abs() > 4 * bound).all() and ((out[0].double() - ref).abs() <= bound).all()
+
+
+# ------------------------------------------------------------------ the checked mode, several callers at once
+def test_checked_calls_report_their_own_errors(monkeypatch):
+    """The device's error word is one for all: a checked call must not clear what another's raised.  The word is a variable here."""
+    import threading
+    import time
+    from flashprefill_b200 import _ops
+    word = []
+
+    class Ext:
+        @staticmethod
+        def paged_decode(q, *rest):
+            time.sleep(0.001)
+            if q.bad:
+                word.append("bad")
+
+    class Q:
+        device = torch.device("cpu")
+
+        def __init__(self, bad):
+            self.bad = bad
+
+    def check(device=None):
+        time.sleep(0.001)
+        found, word[:] = list(word), []
+        if found:
+            raise fp.FlashPrefillError("bad")
+
+    class Anywhere:
+        def __init__(self, device): pass
+        def __enter__(self): pass
+        def __exit__(self, *a): pass
+
+    monkeypatch.setattr(_ops, "CHECK", True)
+    monkeypatch.setattr(_ops, "check_paged_error", check)
+    monkeypatch.setattr(_lib, "_ext", Ext)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "device", Anywhere)
+    raised = {}
+
+    def work(name, bad):
+        n = 0
+        for _ in range(30):
+            try:
+                fp.paged_decode(Q(bad), *[None] * 5)
+            except fp.FlashPrefillError:
+                n += 1
+        raised[name] = n
+
+    threads = [threading.Thread(target=work, args=(i, i % 2 == 0)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert raised == {0: 30, 1: 0, 2: 30, 3: 0}
+
+
+@pytest.mark.gpu
+def test_checked_mode_of_two_threads():
+    """FLASHPREFILL_B200_CHECK=1 in two threads on streams of their own: each call with a slot outside the cache raises, no other."""
+    import subprocess
+    import sys
+    code = """
+import threading, torch, flashprefill_b200 as fp
+r = torch.zeros(2, 1, 128, dtype=torch.bfloat16, device="cuda")
+raised = [0, 0]
+def work(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        c = fp.kv_cache_alloc(4, 16, 1)
+        slots = torch.tensor([1, 3 if i else 64], device="cuda")
+        for _ in range(200):
+            try:
+                fp.kv_cache_write(r, r, c.k, c.v, slots)
+            except fp.FlashPrefillError:
+                raised[i] += 1
+torch.cuda.synchronize()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+print(raised)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, FLASHPREFILL_B200_CHECK="1", PYTHONPATH=root), capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split("\n")[0] == "[200, 0]", r.stdout + r.stderr
