@@ -397,3 +397,45 @@ print(raised)
     r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, FLASHPREFILL_B200_CHECK="1", PYTHONPATH=root), capture_output=True,
                        text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.split("\n")[0] == "[200, 0]", r.stdout + r.stderr
+
+
+# ------------------------------------------------------------------ registered ops
+@pytest.mark.gpu
+@pytest.mark.parametrize("quant", [False, True])
+def test_registered_write_read_and_decode_match_the_entry_points(quant):
+    """A run of the three through torch.ops, eagerly and traced by torch.compile, against the Python entry points."""
+    cd, n = E4M3 if quant else BF16, 100
+    g = torch.Generator(device="cuda").manual_seed(70)
+    k, v = (torch.randn(n, 2, 128, generator=g, device="cuda").to(BF16) for _ in range(2))
+    q = torch.randn(1, 8, 128, generator=g, device="cuda").to(BF16)
+    slots = torch.randperm(128, generator=g, device="cuda")[:n]
+    table, lens = torch.tensor([[3, 1, 7, 0]], dtype=torch.int32, device="cuda"), torch.tensor([60], dtype=torch.int32, device="cuda")
+
+    def run(write, read, decode):
+        c = fp.KVCache(*(None if t is None else t.zero_() for t in fp.kv_cache_alloc(8, 16, 2, cd)))
+        kr, vr, out, lse = (torch.zeros(1, 64, 2, 128, dtype=BF16, device="cuda"), torch.zeros(1, 64, 2, 128, dtype=BF16, device="cuda"),
+                            torch.zeros_like(q), torch.zeros(1, 8, device="cuda"))
+        write(k, v, c.k, c.v, slots, c.k_scale, c.v_scale)
+        read(c.k, c.v, table, lens, kr, vr, c.k_scale, c.v_scale)
+        decode(q, c.k, c.v, table, lens, out, lse, c.k_scale, c.v_scale)
+        return [*(t for t in c if t is not None), kr, vr, out, lse]
+
+    ops = torch.ops.flashprefill
+    want = run(fp.kv_cache_write, fp.kv_cache_read, fp.paged_decode)
+    got = run(ops.kv_cache_write, ops.kv_cache_read, ops.paged_decode)
+    for a, b in zip(got, want):
+        assert same_bits(a, b)
+
+    def traced(kr, vr, out, lse, *cache):
+        ks, vs = cache[2:] if quant else (None, None)
+        ops.kv_cache_write(k, v, cache[0], cache[1], slots, ks, vs)
+        ops.kv_cache_read(cache[0], cache[1], table, lens, kr, vr, ks, vs)
+        ops.paged_decode(q, cache[0], cache[1], table, lens, out, lse, ks, vs)
+        return out * 1.0
+
+    outs = [torch.zeros_like(t) for t in want[-4:]]
+    cache = [t.zero_() for t in fp.kv_cache_alloc(8, 16, 2, cd) if t is not None]
+    torch.compile(traced, backend="aot_eager", fullgraph=True)(*outs, *cache)
+    for a, b in zip(cache + outs, want):
+        assert same_bits(a, b)
+    fp.check_paged_error()
