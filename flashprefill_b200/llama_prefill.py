@@ -147,7 +147,8 @@ class TPLlamaPrefill:
         return x
 
     def _layer(self, L, x, cos, sin, attend):
-        """One layer on the hidden rows x; ``attend(q, k, v)`` on (rows, heads, D) returns the attention as (rows, hq * D)."""
+        """One layer on the hidden rows x, which it updates in place (its caller holds x too: a new tensor would be a second hidden
+        state at the layer's peak); ``attend(q, k, v)`` on (rows, heads, D) returns the attention as (rows, hq * D)."""
         cfg = self.cfg
         S, D = x.shape[0], cfg.head_dim
         nq, nk = self.hq_l * D, self.hk_l * D
@@ -160,7 +161,7 @@ class TPLlamaPrefill:
         attn = attend(q, k, v)
         del q, k, v
         o = attn @ L["wo"].t()
-        x = x + self._reduce(o)
+        x += self._reduce(o)
         del o
         h = rms_norm(x, L["mlp_norm"], cfg.eps)
         gu = h @ L["wgu"].t()
@@ -168,7 +169,8 @@ class TPLlamaPrefill:
         del gu
         y = a @ L["wd"].t()
         del a
-        return x + self._reduce(y)
+        x += self._reduce(y)
+        return x
 
     def _logits(self, x):
         last = rms_norm(x, self.final_norm, self.cfg.eps)
