@@ -33,3 +33,31 @@ def test_layers_leave_the_embedding_alone():
     tokens = torch.arange(cfg.vocab)[-50:]
     first = m.forward(tokens)
     assert torch.equal(m.embed, before) and torch.equal(m.forward(tokens), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 3, 33])
+def test_token_logits_are_summed_in_32_bits_without_a_wide_head(rows, dtype):
+    cfg = LlamaConfig(layers=0, hidden=1024, q_heads=8, kv_heads=2, ffn=2048, vocab=20001)
+    m = TPLlamaPrefill(cfg, device="cuda:0", dtype=dtype, seed=4)
+    x = torch.randn(rows, cfg.hidden, generator=torch.Generator("cuda").manual_seed(rows), device="cuda").to(dtype)
+    m._token_logits(x)  # cuBLAS takes its workspace
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = m._token_logits(x)
+    assert torch.cuda.max_memory_allocated() - before < 2 * m.lm_head.numel()  # bytes: less than a second head, let alone a wide one
+    assert got.dtype is torch.float32 and got.shape == (rows, cfg.vocab)
+    last = x.float()
+    last = (last * torch.rsqrt(last.pow(2).mean(-1, keepdim=True) + cfg.eps)).to(dtype).double()
+    head = m.lm_head.double()
+    # exact products; 1024 of them summed in fp32, each step off by 2^-23 at the most (tensor cores truncate)
+    bound = cfg.hidden * 2.0 ** -23 * (last.abs() @ head.abs().t())
+    assert ((got.double() - last @ head.t()).abs() <= bound).all()
+
+
+def test_token_logits_on_the_cpu_are_the_prompts():
+    m = TPLlamaPrefill(LlamaConfig(**SMALL), device="cpu", dtype=torch.float32, seed=3, attention=dense_causal)
+    x = torch.randn(3, 256, generator=torch.Generator().manual_seed(1))
+    assert torch.equal(m._token_logits(x), m._logits(x))
