@@ -211,6 +211,12 @@ class TPLlamaPrefill:
         return self._logits(x[-1:])[0]
 
     # ------------------------------------------------------------------ with a paged cache (CUDA only)
+    def _refuse_capture(self, what: str) -> None:
+        """The cache counts its tokens on the host too: a replay would leave that count behind and pass its checks, until a position
+        beyond the cache ends in a device-side assert."""
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} counts tokens on the host and cannot be captured in a CUDA graph")
+
     def new_cache(self, batch: int, max_len: int, page_size: int = 64, dtype: torch.dtype | None = None) -> LlamaCache:
         """An empty cache for ``batch`` sequences of up to ``max_len`` tokens; ``dtype``: the model's, or
         torch.float8_e4m3fn."""
@@ -224,9 +230,11 @@ class TPLlamaPrefill:
     @torch.no_grad()
     def prefill(self, tokens: torch.Tensor, cache: LlamaCache, seq: int = 0) -> torch.Tensor:
         """Append the token ids (S,) to sequence ``seq`` of the cache and return the last one's logits (vocab,) in fp32.
-        Tokens after the first chunk attend to the cached prefix, read back, and to their own keys."""
+        Tokens after the first chunk attend to the cached prefix, read back, and to their own keys.  Not to be captured in a CUDA
+        graph (refused), as the cache counts on the host."""
         from .paged_cache import kv_cache_read, kv_cache_write
         cfg = self.cfg
+        self._refuse_capture("prefill")
         if not 0 <= seq < len(cache.lens):
             raise ValueError(f"sequence {seq} of the cache's {len(cache.lens)}")
         S, D, n = tokens.shape[0], cfg.head_dim, cache.lens[seq]
@@ -259,9 +267,11 @@ class TPLlamaPrefill:
 
     @torch.no_grad()
     def decode(self, tokens: torch.Tensor, cache: LlamaCache) -> torch.Tensor:
-        """One new token id for each sequence of the cache, (batch,); returns the logits (batch, vocab) in fp32."""
+        """One new token id for each sequence of the cache, (batch,); returns the logits (batch, vocab) in fp32.  Not to be captured
+        in a CUDA graph (refused), as the cache counts on the host."""
         from .paged_cache import kv_cache_write, paged_decode
         cfg = self.cfg
+        self._refuse_capture("decode")
         B, D = tokens.shape[0], cfg.head_dim
         if B != len(cache.lens):
             raise ValueError(f"{B} tokens for the cache's {len(cache.lens)} sequences")

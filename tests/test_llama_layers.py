@@ -61,3 +61,15 @@ def test_token_logits_on_the_cpu_are_the_prompts():
     m = TPLlamaPrefill(LlamaConfig(**SMALL), device="cpu", dtype=torch.float32, seed=3, attention=dense_causal)
     x = torch.randn(3, 256, generator=torch.Generator().manual_seed(1))
     assert torch.equal(m._token_logits(x), m._logits(x))
+
+
+def test_cached_steps_refuse_to_be_captured(monkeypatch):
+    m = TPLlamaPrefill(LlamaConfig(**SMALL), device="cpu", dtype=torch.float32, seed=3, attention=dense_causal)
+    cache = m.new_cache(2, 64, page_size=16, dtype=torch.bfloat16)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="prefill .*captured"):
+        m.prefill(torch.zeros(3, dtype=torch.int64), cache)
+    with pytest.raises(RuntimeError, match="decode .*captured"):
+        m.decode(torch.zeros(2, dtype=torch.int64), cache)
+    assert cache.lens == [0, 0]
