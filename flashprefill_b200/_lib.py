@@ -116,10 +116,14 @@ def ext():
                 import importlib.machinery
                 import importlib.util
 
-                import torch  # noqa: F401  (its libraries must be loaded first)
+                import torch  # its libraries must be loaded first
                 loader = importlib.machinery.ExtensionFileLoader("_fp_torch", EXT_PATH)
                 m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fp_torch", loader))
                 loader.exec_module(m)
+                if m.built_for != torch.__version__:
+                    raise ImportError(
+                        f"flashprefill_b200: torch binding built for torch {m.built_for}, this is {torch.__version__}; run "
+                        "`python -m flashprefill_b200.build`")
                 addr = lambda name: ctypes.cast(getattr(lib, name), _P).value
                 m.bind(addr("fpb_kv_cache_write"), addr("fpb_kv_cache_read"), addr("fpb_paged_decode"),
                        addr("fpb_paged_decode_workspace_bytes"), addr("fpb_last_error"), FlashPrefillError)

@@ -3,8 +3,9 @@
     python -m flashprefill_b200.build [--verbose-ptxas]
 
 The library is one unity translation unit (csrc/fp_api.cu includes the kernels) linked
-against the static CUDA runtime, so it only needs the NVIDIA driver at run time.  Beside it
-_fp_torch.so (csrc/fp_torch.cpp, g++) passes torch tensors to the paged-cache entry points.
+against the static CUDA runtime, so it only needs the NVIDIA driver at run time.  Behind it
+_fp_torch.so (csrc/fp_torch.cpp, g++) is built, which passes torch tensors to the paged-cache entry
+points; it goes by the torch that it was built for, and C callers do not need it.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libflashprefill_b200.so")
 SOURCES = ["fp_api.cu"]
 EXT = os.path.join(HERE, "_fp_torch.so")
+EXT_TAG = EXT + ".built_for"
 EXT_SOURCE = "fp_torch.cpp"
 HEADER = os.path.join(os.path.dirname(HERE), "include", "flashprefill_b200.h")
 
@@ -42,18 +44,37 @@ def needs_build() -> bool:
     return any(os.path.getmtime(d) > t for d in _deps())
 
 
+def _ext_tag() -> str:
+    """What _fp_torch.so depends on beside its source: torch's C++ interface and Python's."""
+    import sysconfig
+
+    import torch
+    return f"{torch.__version__} {sysconfig.get_config_var('SOABI')}"
+
+
+def ext_needs_build() -> bool:
+    src = os.path.join(CSRC, EXT_SOURCE)
+    if not (os.path.exists(EXT) and os.path.exists(EXT_TAG)):
+        return True
+    if any(os.path.getmtime(d) >= os.path.getmtime(EXT) for d in (src, HEADER)):
+        return True
+    with open(EXT_TAG) as f:
+        return f.read() != _ext_tag()
+
+
 def build_ext(force: bool = False) -> str:
     """_fp_torch.so: plain g++ against torch's headers (its C++ interface has no device code)."""
-    src = os.path.join(CSRC, EXT_SOURCE)
-    if not force and os.path.exists(EXT) and all(os.path.getmtime(EXT) > os.path.getmtime(d) for d in (src, HEADER)):
+    if not force and not ext_needs_build():
         return EXT
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
+    src = os.path.join(CSRC, EXT_SOURCE)
     cuda = os.path.dirname(os.path.dirname(nvcc_path()))
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", EXT + ".tmp", src]
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DFPB_BUILT_FOR="{torch.__version__}"',
+           "-o", EXT + ".tmp", src]
     for d in cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]:
         cmd += ["-isystem", d]
     for d in cpp_extension.library_paths():
@@ -63,11 +84,18 @@ def build_ext(force: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError("g++ failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
     os.replace(EXT + ".tmp", EXT)
+    with open(EXT_TAG, "w") as f:
+        f.write(_ext_tag())
     return EXT
 
 
 def build(force: bool = False, ptxas_verbose: bool = False) -> str:
+    lib = build_lib(force, ptxas_verbose)  # first: it needs neither g++ nor torch's headers
     build_ext(force)
+    return lib
+
+
+def build_lib(force: bool = False, ptxas_verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB
     cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",

@@ -301,4 +301,8 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_fp_torch", nullptr, -1, g_metho
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__fp_torch() { return PyModule_Create(&g_module); }
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__fp_torch() {
+  PyObject* m = PyModule_Create(&g_module);
+  if (m && PyModule_AddStringConstant(m, "built_for", FPB_BUILT_FOR) < 0) Py_CLEAR(m);  // torch.__version__
+  return m;
+}
