@@ -13,7 +13,7 @@ from ._ops import (check_device_error, check_paged_error, get_mean_warps, paged_
 from .flashprefill_native_forward import flash_prefill
 from .flashprefill_varlen_func import flash_prefill_varlen_func
 from .paged_cache import KVCache, kv_cache_alloc, kv_cache_read, kv_cache_write, paged_decode
-from . import torch_ops  # registers torch.ops.flashprefill.prefill_dense / prefill_varlen
+from . import torch_ops  # registers torch.ops.flashprefill.*
 
 __all__ = ["flash_prefill", "flash_prefill_varlen_func", "search_dense", "search_varlen", "set_mean_warps",
            "get_mean_warps", "check_device_error", "FlashPrefillError", "install_as_ops", "KVCache", "kv_cache_alloc",

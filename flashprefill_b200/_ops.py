@@ -20,7 +20,7 @@ _DTYPES = {torch.bfloat16: _lib.FPB_BF16, torch.float16: _lib.FPB_FP16}
 # (the reference's autotuner picks 4 or 8, ops/flashprefill_native_forward.py:7-20).
 _MEAN_WARPS = int(os.environ.get("FLASHPREFILL_B200_MEAN_WARPS", "4"))
 # When set, every call synchronises and raises if a kernel reported a device error.
-CHECK = _CHECK = os.environ.get("FLASHPREFILL_B200_CHECK", "0") not in ("", "0")
+CHECK = os.environ.get("FLASHPREFILL_B200_CHECK", "0") not in ("", "0")
 
 LAYOUT_KEYS = ["err", "cu_tile", "mk", "cnt", "idx", "total", "tiles", "cap"]
 
@@ -72,7 +72,7 @@ def _P(x):
 
 
 def _finish(ws: torch.Tensor, stream) -> None:
-    if _CHECK:
+    if CHECK:
         check_device_error(ws, stream)
 
 

@@ -4,8 +4,8 @@
 //   s_j = sm_scale * q . k_j,   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   lse = m + log sum_j exp(s_j - m)
 //
 // for every sequence b and query head, j over the sequence's seq_lens[b] cached tokens; the G = hq / hk query heads of a
-// KV head share its rows.  Each cached byte is read once and meets G flops (2-byte cache) or 2 G (e4m3), so the operator is
-// bound by HBM; the arithmetic only has to stay out of the way.
+// KV head share its rows.  Each cached byte is read once (once for each group of at most 16 heads, where a KV head has more) and
+// meets G flops (2-byte cache) or 2 G (e4m3), so the operator is bound by HBM; the arithmetic only has to stay out of the way.
 //
 // An item is (sequence, KV head, group of query heads: all G up to 16, equal groups of at most 16 above that); its tokens are
 // cut into units of TT tokens for each warp of a CTA.  Lengths are read on the device (no host copy; a captured graph serves
@@ -17,7 +17,8 @@
 // leaves unnormalised sums and their maxima in the workspace; a second kernel joins them in the order of the tokens.
 // Short sequences (paged_decode_short_kernel): one cluster of 1 to 8 CTAs for each item, units dealt out in turn, joined
 // through distributed shared memory.  No prefix sums, no workspace, no second kernel.
-// Both join in an order that the lengths alone decide, with no atomics: the same call gives the same bits.
+// Both join in an order that follows from the call's shapes (the table's width among them) and the lengths, with no atomics: the
+// same call gives the same bits.
 //
 // A warp works alone on its own tiles of TT tokens (16 of a 16-bit cache, 32 of e4m3: 4 KB of K and of V each way) through
 // a ring of kDecStages tiles filled by 16-byte cp.async, so loads are in flight all the time without block-wide barriers;
@@ -44,12 +45,12 @@
 //     (With weights relative to the largest score and V scales to the largest of any token, a row of small values behind one of
 //     large values lost bits, and all of them from 2^39 on, even where the softmax gave the large ones no weight.)
 //
-// Measured (device time; of the measured 6.54 TB/s): 64 x up to 8192 tokens of 32/8 heads, bf16, 1.11 GB, 163 to 169 us (100%
-// and more: reads alone pass a copy's rate); 1 x 131072, 0.54 GB, 86 us (95%); 2 x up to 262144 of 28/4 heads, e4m3, 0.53 GB,
-// 83 to 87 us (93 to 97%), 46% of the issue slots; 33 x up to 16001 of 28/4 heads, e4m3, 0.31 GB, 53 to 57 us (82 to 88%): 3 us
-// from the launch to the first full stream (lengths, table, rows: three loads in turn), 3 us between the first CTA that ends
-// and the last, 4 us for the join.  1 x 500 of 32/8 heads, 2 MB, 4.5 us: the launch 0.9, the same loads in turn and the warps'
-// sums 1.8, the cluster's barrier and sums 1.8.
+// Measured (calls in a row; of the measured 6.54 TB/s): 64 x up to 8192 tokens of 32/8 heads, bf16, 1.11 GB, 165 us (100%
+// and more: reads alone pass a copy's rate); 1 x 131072, 0.54 GB, 84 us (98%); 2 x up to 262144 of 28/4 heads, e4m3, 0.53 GB,
+// 88 us (92%; 82 at the clocks of a short run), 52% of the issue slots; 33 x up to 16001 of 28/4 heads, e4m3, 0.31 GB, 57.5 us
+// (81%; 53 at the clocks of a short run): 3 us from the launch to the first full stream (lengths, table, rows: three loads in
+// turn), 3 us between the first CTA that ends and the last, 4 us for the join.  1 x 500 of 32/8 heads, 2 MB, 4.5 us: the launch
+// 0.9, the same loads in turn and the warps' sums 1.8, the cluster's barrier and sums 1.8.
 #include <type_traits>
 
 #include "fp_common.cuh"
@@ -91,7 +92,8 @@ struct DecodeArgs {
 };
 
 // 16 bytes of the cache (`bytes` of them, then zeros) to shared memory.  Cached rows pass through L2 once: evicted first, they
-// leave it to the tables, lengths and partial sums (28/4 heads, 33 x up to 16001 tokens of e4m3: 57 us without, 53 with).
+// leave it to the tables, lengths and partial sums (28/4 heads, 33 x up to 16001 tokens of e4m3, one part of each weight: 57 us
+// without, 53 with).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   uint64_t policy;
   asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));

@@ -52,7 +52,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
                    k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
     """Write rows k, v (T, kv_heads, 128) into the cache slots ``slots`` (T,), int64 or int32; a negative slot skips its row.
 
-    An e4m3 cache gets ``scale = max(max|x|, 2**-100) / 448`` and codes ``x / scale`` for each row; a row with an infinity or
+    An e4m3 cache gets ``scale = max(max|x|, 2**-100) / 448`` and codes ``x * (448 / max(max|x|, 2**-100))`` for each row; a row with an infinity or
     a NaN reads back as NaN.  k and v may have any strides (e.g. columns of a fused projection; copied only where rows are not
     16-byte aligned).  The slots of one call must differ from one another (FLASHPREFILL_B200_CHECK=1 checks that); where two
     rows name one slot, its contents are not defined.  k_cache and v_cache must be different memory, as must the scales."""
@@ -87,7 +87,8 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     16-bit cache keep to the softmax (any weight makes the channel infinite; a weight that vanishes, below 2^-39 of the largest
     for float16 and 2^-100 for bfloat16, makes it NaN, as 0 times infinity).  ``sm_scale`` is 1/sqrt(128) by default.  ``workspace``: uint8 of at least ``paged_decode_workspace_bytes``, taken from the caching
     allocator by default; calls that may overlap on the GPU (other streams, graphs replayed side by side) need one each.
-    Results do not depend on the order in which the GPU runs its blocks: the same call gives the same bits."""
+    Results do not depend on the order in which the GPU runs its blocks: the same call gives the same bits (the same sequences
+    behind a table of another width may be split, and rounded, in another way)."""
     decode = (_lib._ext or _lib.ext()).paged_decode
     if _ops.CHECK:
         return _ops.checked_paged(decode, (q, k_cache, v_cache, page_table, seq_lens, out, lse, k_scale, v_scale, sm_scale, workspace))

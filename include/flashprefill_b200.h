@@ -248,7 +248,8 @@ FPB_API int fpb_kv_cache_read(const void* k_cache, const void* v_cache, int cach
                               int64_t table_stride, int max_pages, const int32_t* seq_lens, int batch, void* k, void* v,
                               int dtype, int out_len, const int64_t* k_strides, const int64_t* v_strides, void* stream);
 
-/* Workspace of fpb_paged_decode (0 where none is needed: sequences of at most one unit of work). */
+/* Workspace of fpb_paged_decode.  It follows from the batch, the heads and the table's width, max_pages * page_size (not from the
+ * lengths), and is 0 where sequences of that width are short enough to be joined in shared memory. */
 FPB_API size_t fpb_paged_decode_workspace_bytes(int batch, int hq, int hk, int cache_dtype, int max_pages,
                                                 int page_size);
 
