@@ -42,8 +42,9 @@
 //   * e4m3: codes widen to fp16 exactly; q is scaled by a power of two to fill fp16's range; the token's K scale multiplies its
 //     score and its V scale its weight.  These products must fit fp16, so the running maximum is that of score + log2(V scale)
 //     and they reach 2^15; the sum of the weights goes by the same reference and is brought to [1, 2) when an item ends.
-//     (With weights relative to the largest score and V scales to the largest of any token, a row of small values behind one of
-//     large values lost bits, and all of them from 2^39 on, even where the softmax gave the large ones no weight.)
+//     With weights relative to the largest score and V scales to the largest of any token, a row of small values behind one of
+//     large values lost bits, and all of them from 2^39 on, even where the softmax gave the large ones no weight.  Scores
+//     beyond 4096 need another reference (weigh_large); a warp that meets one begins its item again.
 //
 // Measured (calls in a row; of the measured 6.54 TB/s): 64 x up to 8192 tokens of 32/8 heads, bf16, 1.11 GB, 165 us (100%
 // and more: reads alone pass a copy's rate); 1 x 131072, 0.54 GB, 84 us (98%); 2 x up to 262144 of 28/4 heads, e4m3, 0.53 GB,
@@ -51,6 +52,7 @@
 // (81%; 53 at the clocks of a short run): 3 us from the launch to the first full stream (lengths, table, rows: three loads in
 // turn), 3 us between the first CTA that ends and the last, 4 us for the join.  1 x 500 of 32/8 heads, 2 MB, 4.5 us: the launch
 // 0.9, the same loads in turn and the warps' sums 1.8, the cluster's barrier and sums 1.8.
+#include <cfloat>
 #include <type_traits>
 
 #include "fp_common.cuh"
@@ -190,6 +192,7 @@ struct DecodeWarp {
   static constexpr int kChunks = kRowBytes / 16;  // 16-byte pieces of a row
   static constexpr uint32_t kFull = TT == 32 ? 0xFFFFFFFFu : 0xFFFFu;
   static constexpr float kShift = DT<MT>::is_bf16 ? 0.f : 15.f;  // log2 of the factor of P and l
+  static constexpr float kLarge = 4096.f;                        // e4m3: scores beyond are weighed by weigh_large
   // V scales as the running maximum takes them: P is kept finite beyond, and the sum of 2^31 weights below.
   static constexpr float kLeastScale = 8.271806125530277e-25f;   // 2^-80
   static constexpr float kLargestScale = 1.329227995784916e36f;  // 2^120
@@ -349,11 +352,36 @@ struct DecodeWarp {
     }
   }
 
-  __device__ __forceinline__ void consume(int stage, uint32_t valid) {
-    const uint32_t kd = ring + stage * kDecStageBytes, vd = kd + kDecTileBytes;
-    const int g = lane >> 2;
-    const uint32_t ksd = kd + 2 * kDecTileBytes, vsd = ksd + kDecScaleBytes;
-    float s[NT][MTILES][4];
+  // Scales of the row of a tile that this thread's elements (i, h) of s belong to: g + 8 h + 16 i.
+  __device__ __forceinline__ float k_scale(int stage, int i, int h) const {
+    return lds(ring + stage * kDecStageBytes + 2 * kDecTileBytes + 4 * (16 * i + 8 * h + (lane >> 2)));
+  }
+  __device__ __forceinline__ float v_scale(int stage, int i, int h) const {
+    return lds(ring + stage * kDecStageBytes + 2 * kDecTileBytes + kDecScaleBytes + 4 * (16 * i + 8 * h + (lane >> 2)));
+  }
+  __device__ __forceinline__ float log_v_scale(int stage, int i, int h) const {
+    return __log2f(fminf(fmaxf(fabsf(v_scale(stage, i, h)), kLeastScale), kLargestScale));
+  }
+  // Whether that row is there.
+  __device__ __forceinline__ bool there(uint32_t valid, int i, int h) const { return (valid >> (16 * i + 8 * h + (lane >> 2))) & 1u; }
+  // The largest of a column's rows.
+  static __device__ __forceinline__ float max_rows(float x) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+  }
+  __device__ __forceinline__ void rescale(int n, float (&f)[2]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) l[n][j] *= f[j];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[n][i][j] *= f[j & 1];
+  }
+
+  // Products of a tile's keys and q, times the factor of q: scores in log2 units, of an e4m3 row without its K scale.
+  __device__ __forceinline__ void scores(int stage, float (&s)[NT][MTILES][4]) {
+    const uint32_t kd = ring + stage * kDecStageBytes;
     {
       float s2[NT][4];  // second chain of products of a 16-token tile (32 tokens have two as it is)
 #pragma unroll
@@ -391,28 +419,34 @@ struct DecodeWarp {
           for (int j = 0; j < 4; ++j) s[n][0][j] += s2[n][j];
       }
     }
-    // scores in log2 units
 #pragma unroll
-    for (int i = 0; i < MTILES; ++i)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float kf = 1.f;
-        if constexpr (kE4m3) kf = lds(ksd + 4 * (16 * i + 8 * h + g));
+      for (int i = 0; i < MTILES; ++i)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int j = 0; j < 4; ++j) s[n][i][j] *= qc[n][j & 1];
+  }
+
+  // Scores of a tile to weights.  e4m3: false, with nothing done, where the running maximum would leave [-kLarge, kLarge].
+  __device__ __forceinline__ bool weigh(int stage, uint32_t valid, float (&s)[NT][MTILES][4]) {
+    if constexpr (kE4m3) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float& x = s[n][i][2 * h + j];
-            x *= qc[n][j];
-            if constexpr (kE4m3) x *= kf;
-          }
-      }
+      for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float kf = k_scale(stage, i, h);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s[n][i][2 * h + j] *= kf;
+        }
+    }
     if (valid != kFull) {
 #pragma unroll
       for (int i = 0; i < MTILES; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if (!((valid >> (16 * i + 8 * h + g)) & 1u)) {
+          if (!there(valid, i, h)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) s[n][i][2 * h] = s[n][i][2 * h + 1] = -INFINITY;
           }
@@ -423,8 +457,7 @@ struct DecodeWarp {
     for (int i = 0; i < MTILES; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float lv = 0.f;
-        if constexpr (kE4m3) lv = __log2f(fminf(fmaxf(fabsf(lds(vsd + 4 * (16 * i + 8 * h + g))), kLeastScale), kLargestScale));
+        const float lv = kE4m3 ? log_v_scale(stage, i, h) : 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -437,41 +470,95 @@ struct DecodeWarp {
 #pragma unroll
     for (int n = 0; n < NT; ++n) moved |= mx[n][0] > m[n][0] || mx[n][1] > m[n][1];
     if (__any_sync(0xffffffffu, moved)) {
+      bool large = false;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float corr[2];
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float x = mx[n][j];
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-          const float mn = fmaxf(m[n][j], x), f = ex2_approx(m[n][j] - finite_or_zero(mn));
-          m[n][j] = mn;
-          l[n][j] *= f;
-          corr[j] = f;
+          mx[n][j] = fmaxf(m[n][j], max_rows(mx[n][j]));
+          large |= fabsf(finite_or_zero(mx[n][j])) > kLarge;
         }
+      if (kE4m3 && __any_sync(0xffffffffu, large)) return false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+      for (int n = 0; n < NT; ++n) {
+        float f[2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o[n][i][j] *= corr[j & 1];
+        for (int j = 0; j < 2; ++j) {
+          f[j] = ex2_approx(m[n][j] - finite_or_zero(mx[n][j]));
+          m[n][j] = mx[n][j];
+        }
+        rescale(n, f);
       }
     }
+#pragma unroll
+    for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float& x = s[n][i][2 * h + j];
+            x = ex2_approx(kE4m3 ? x - (finite_or_zero(m[n][j]) - kShift) : (x - finite_or_zero(m[n][j])) + kShift);
+            l[n][j] += x;
+          }
+    return true;
+  }
+
+  // The same for e4m3 scores of any size.  Above some millions what is added to a score is rounded away, so the reference has two
+  // parts, m + w: m the largest score, w the log2 that the largest product of a weight and a V scale has above it, less kShift.
+  // Scores are taken off m with one rounding.  (In every tile this would cost 33 x 16K 2 us of 53.)
+  __device__ __forceinline__ void weigh_large(int stage, uint32_t valid, float (&s)[NT][MTILES][4], float (&w)[NT][2]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float f[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float x = m[n][j], y = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (there(valid, i, h)) x = fmaxf(x, s[n][i][2 * h + j] * k_scale(stage, i, h));
+        x = max_rows(x);
+        const float up = x - m[n][j];
+#pragma unroll
+        for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float& d = s[n][i][2 * h + j];
+            d = there(valid, i, h) ? fmaf(d, k_scale(stage, i, h), -x) : -INFINITY;
+            y = fmaxf(y, d + log_v_scale(stage, i, h));
+          }
+        const float wn = fmaxf(w[n][j] - up, max_rows(y) - kShift);
+        f[j] = ex2_approx(w[n][j] - up - wn);
+        m[n][j] = x;
+        w[n][j] = wn;
+#pragma unroll
+        for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) s[n][i][2 * h + j] = ex2_approx(s[n][i][2 * h + j] - wn);
+      }
+      rescale(n, f);
+#pragma unroll
+      for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l[n][j & 1] += s[n][i][j];
+    }
+  }
+
+  // Weights times the tile's values.
+  __device__ __forceinline__ void products(int stage, const float (&s)[NT][MTILES][4]) {
+    const uint32_t vd = ring + stage * kDecStageBytes + kDecTileBytes;
     uint32_t pb[NT][MTILES][2], pl[NT][MTILES][2];
 #pragma unroll
     for (int i = 0; i < MTILES; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float vs = 1.f;
-        if constexpr (kE4m3) vs = lds(vsd + 4 * (16 * i + 8 * h + g));
+        const float vs = kE4m3 ? v_scale(stage, i, h) : 1.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float p[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            p[j] = ex2_approx(s[n][i][2 * h + j] - (finite_or_zero(m[n][j]) - kShift));
-            l[n][j] += p[j];
-            if constexpr (kE4m3) p[j] *= vs;
-          }
+          const float p[2] = {s[n][i][2 * h] * vs, s[n][i][2 * h + 1] * vs};
           uint32_t hi, lo;
           if constexpr (!kE4m3) {
             split_weights<MT>(p[0], p[1], hi, lo);
@@ -511,6 +598,15 @@ struct DecodeWarp {
         }
       }
     }
+  }
+
+  // False where weigh refused: the item's scores are large.
+  __device__ __forceinline__ bool consume(int stage, uint32_t valid) {
+    float s[NT][MTILES][4];
+    scores(stage, s);
+    if (!weigh(stage, valid, s)) return false;
+    products(stage, s);
+    return true;
   }
 
   // All of this warp's tiles of an item: tokens [tok + i * step, + TT) below min(end, the sequence's length).  The first
@@ -560,13 +656,50 @@ struct DecodeWarp {
             cp_async_wait<kDecStages - 1>();
             __syncwarp();
           }
-          consume(j, valid[j]);
+          if (!consume(j, valid[j])) goto large;
           __syncwarp();
         }
       }
     }
     cp_async_wait<0>();
     __syncwarp();
+    return;
+  large:
+    if constexpr (kE4m3) {  // once more from the first tile, one after another
+      cp_async_wait<0>();
+      __syncwarp();
+      reset();
+      float w[NT][2];
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) m[k][j] = w[k][j] = -FLT_MAX;
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        load_pages(A, table, tok + i * step, page);
+        issue(A, table, h, tok + i * step, end, 0, page, valid[0]);
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncwarp();
+        float s[NT][MTILES][4];
+        scores(0, s);
+        weigh_large(0, valid[0], s, w);
+        products(0, s);
+        __syncwarp();
+      }
+      // sums relative to m, as scores are: what is added to m now would be rounded away
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        float f[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool none = w[k][j] == -FLT_MAX;
+          f[j] = none ? 1.f : ex2_approx(w[k][j] + kShift);
+          if (none) m[k][j] = -INFINITY;
+        }
+        rescale(k, f);
+      }
+    }
   }
 
   // Sums and maxima into shared memory: rows of 132 floats for each head (conflict-free), {maximum, sum} beside them.
@@ -580,10 +713,15 @@ struct DecodeWarp {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
         const int h = n * 8 + 2 * t + j;
-        int e = 0;
-        if constexpr (kE4m3) e = max(-120, min((int)(__float_as_uint(x) >> 23) - 127, 120));
-        const float f = exp2i(-e);
-        if (g == 0) sml[h] = make_float2(m[n][j] - kShift + (float)e, x * f);
+        // relative to m: the factor 2^kShift comes off the sums, not m.  e4m3 sums of scores that are not large are first brought
+        // to [1, 2), as they may be far from it.
+        float f = exp2i(-(int)kShift), top = m[n][j];
+        if (kE4m3 && fabsf(top) <= kLarge) {
+          const int e = max(-120, min((int)(__float_as_uint(x) >> 23) - 127, 120));
+          f = exp2i(-e);
+          top += (float)e - kShift;
+        }
+        if (g == 0) sml[h] = make_float2(top, x * f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int d0 = 16 * i + (kE4m3 ? 2 * g : g), d1 = 16 * i + (kE4m3 ? 2 * g + 1 : g + 8);

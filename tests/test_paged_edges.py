@@ -439,3 +439,67 @@ def test_registered_write_read_and_decode_match_the_entry_points(quant):
     for a, b in zip(cache + outs, want):
         assert same_bits(a, b)
     fp.check_paged_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [0, 70000])
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_scores_of_millions_and_more(dtype, quant, room):
+    """Scores whose steps in fp32 are whole powers of two: the tokens of the largest share the weight, all others have none.  Scores are
+    exact products of one channel, so equal ones are equal."""
+    cd = E4M3 if quant else dtype
+    n = 200
+    f = pu.fill_sequences([n] * 6, 4, 1, dtype, cd, 16, seed=80, room=room)
+    f["q"][:] = 0
+    size = torch.tensor([2.0 ** 20, 2.0 ** 22, 2.0 ** 24, 2.0 ** 27, -2.0 ** 24, 2.0 ** 32], dtype=torch.float64)
+    g = torch.Generator().manual_seed(1)
+    for b in range(6):
+        # keys of 1 to 15 in one channel, the query's value times sm_scale 1 gives the size
+        value = torch.randint(1, 16, (n,), generator=g).double().cuda()
+        at = torch.arange(n, device="cuda")
+        page, at = f["page_table"][b].long()[at // 16], at % 16
+        k = torch.zeros(n, 1, 128, dtype=torch.float64, device="cuda")
+        gain = 2.0 ** (10 if quant else 0)
+        k[:, 0, 5] = value * (1.0 if quant else 2.0 ** 10)
+        if quant:
+            f["k"].view(torch.uint8)[page, at] = k.to(E4M3).view(torch.uint8)
+            f["k_scale"][page, at] = gain
+        else:
+            f["k"][page, at] = k.to(cd)
+        f["rows"][b][0][:] = k * gain
+        f["q"][b, :, 5] = (size[b] * 2.0 ** -24).to(dtype)  # 2^-4 to 2^8; the sm_scale below has the rest
+    scale = 2.0 ** 14
+    out, lse = torch.empty_like(f["q"]), torch.empty(6, 4, device="cuda")
+    fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], out, lse, f["k_scale"], f["v_scale"], sm_scale=scale)
+    fp.check_paged_error()
+    for b, (k, v) in enumerate(f["rows"]):
+        ref, rl, weight, _ = pu.attend64(f["q"][b], k, v, scale)
+        to, _ = pu.decode_bounds(ref, rl, weight, torch.zeros_like(rl), n, dtype, cd, f["q"][b] * 0, k, v, scale)
+        err = (out[b].double() - ref).abs()
+        assert (err <= to).all(), (b, (err / to).max().item())
+        # the product with sm_scale * log2(e) and its way back, each off by 2^-24
+        assert ((lse[b].double() - rl).abs() <= 2.0 ** -21 * rl.abs() + 2.0 ** -20).all(), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [0, 70000])
+@pytest.mark.parametrize("hq,page_size", [(8, 16), (24, 5), (24, 48)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_one_head_of_large_scores_beside_ordinary_ones(dtype, hq, page_size, room):
+    """A quantised cache where one head's scores reach tens of thousands, at some place in the sequence: it and its neighbours in the
+    same warps keep to the definition, as does a sequence with none."""
+    f = pu.fill_sequences([3000, 0, 65, 900, 1], hq, 2, dtype, E4M3, page_size, "nhd", seed=81, room=room)
+    f["q"][0, 1] *= 4000.0
+    f["q"][2, hq - 1] *= -3000.0
+    at = 777
+    page, off = f["page_table"][3, at // page_size].long(), at % page_size
+    f["k_scale"][page, off] *= 5000.0  # one token whose key is large for every head
+    f["rows"][3][0][at] = f["k"].view(torch.uint8)[page, off].view(E4M3).double() * f["k_scale"][page, off].double()[:, None]
+    out, lse = torch.full_like(f["q"], float("nan")), torch.full((5, hq), float("nan"), device="cuda")
+    fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], out, lse, f["k_scale"], f["v_scale"])
+    fp.check_paged_error()
+    check_decode(f, out, lse, dtype, E4M3)
+    again = torch.empty_like(out)
+    fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], again, None, f["k_scale"], f["v_scale"])
+    assert same_bits(out, again)
