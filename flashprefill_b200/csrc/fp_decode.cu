@@ -475,7 +475,10 @@ struct DecodeWarp {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          mx[n][j] = fmaxf(m[n][j], max_rows(mx[n][j]));
+          mx[n][j] = max_rows(mx[n][j]);
+          // e4m3: on a grid of 2^-6, so that neither 15 nor the sum's exponent changes its low bits on the way to the lse
+          if constexpr (kE4m3) mx[n][j] = ceilf(mx[n][j] * 64.f) * (1.f / 64.f);
+          mx[n][j] = fmaxf(m[n][j], mx[n][j]);
           large |= fabsf(finite_or_zero(mx[n][j])) > kLarge;
         }
       if (kE4m3 && __any_sync(0xffffffffu, large)) return false;

@@ -503,3 +503,17 @@ def test_one_head_of_large_scores_beside_ordinary_ones(dtype, hq, page_size, roo
     again = torch.empty_like(out)
     fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], again, None, f["k_scale"], f["v_scale"])
     assert same_bits(out, again)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_lse_does_not_depend_on_the_scale_of_the_values(dtype):
+    """Short rows of small scores over a quantised cache: the log of the sum is as near as a 16-bit cache's, for values of any size."""
+    f = pu.fill_sequences([1, 2, 3, 5, 17] * 40, 24, 2, dtype, E4M3, 16, seed=91, k_gain=0.01)
+    f["v_scale"] *= torch.exp2(torch.randint(-6, 7, f["v_scale"].shape, generator=torch.Generator("cuda").manual_seed(1), device="cuda").float())
+    out, lse = torch.empty_like(f["q"]), torch.empty(200, 24, device="cuda")
+    fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], out, lse, f["k_scale"], f["v_scale"], sm_scale=0.01)
+    for b, (k, v) in enumerate(f["rows"]):
+        ref, rl, weight, size = pu.attend64(f["q"][b], k, v, 0.01)
+        _, tl = pu.decode_bounds(ref, rl, weight, size, k.shape[0], dtype, E4M3, f["q"][b], k, v, 0.01)
+        assert ((lse[b].double() - rl).abs() <= tl).all(), (b, ((lse[b].double() - rl).abs() / tl).max().item())
