@@ -354,6 +354,8 @@ def checked_paged(call, args, slots=None) -> None:
 
 
 def paged_decode_workspace_bytes(batch, q_heads, kv_heads, cache_dtype, max_pages, page_size) -> int:
-    """Bytes of workspace that paged_decode needs for these sizes."""
-    code = _lib.FPB_E4M3 if cache_dtype is torch.float8_e4m3fn else _DTYPES[cache_dtype]
+    """Bytes of workspace that paged_decode needs for these sizes (0: none)."""
+    code = _lib.FPB_E4M3 if cache_dtype is torch.float8_e4m3fn else _DTYPES.get(cache_dtype)
+    if code is None:
+        raise TypeError(f"a cache holds bfloat16, float16 or float8_e4m3fn (got {cache_dtype})")
     return _lib.load().fpb_paged_decode_workspace_bytes(batch, q_heads, kv_heads, code, max_pages, page_size)

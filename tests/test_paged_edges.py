@@ -505,6 +505,22 @@ def test_one_head_of_large_scores_beside_ordinary_ones(dtype, hq, page_size, roo
     assert same_bits(out, again)
 
 
+# ------------------------------------------------------------------ refusals
+def test_workspace_of_a_type_that_no_cache_holds_is_refused(lib):
+    with pytest.raises(TypeError, match="float32"):
+        fp.paged_decode_workspace_bytes(1, 8, 2, torch.float32, 64, 16)
+
+
+@pytest.mark.gpu
+def test_a_scale_that_is_no_number_is_refused():
+    f = pu.fill_sequences([20], 4, 2, BF16, BF16, 16, seed=90)
+    for bad in ("0.1", [0.1], object()):
+        with pytest.raises(TypeError):
+            fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], torch.empty_like(f["q"]), sm_scale=bad)
+    with pytest.raises(ValueError, match="sm_scale"):
+        fp.paged_decode(f["q"], f["k"], f["v"], f["page_table"], f["lens"], torch.empty_like(f["q"]), sm_scale=1e300)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_lse_does_not_depend_on_the_scale_of_the_values(dtype):
