@@ -32,8 +32,9 @@
 //   * Scores, maxima, sums and outputs stay in fp32 registers.  The running maximum is reduced over the warp, and sums are
 //     rescaled, only in tiles where some score exceeds it.
 //   * P is split into two 16-bit parts (the value and its remainder) and multiplied twice: one part alone would leave errors
-//     as large as the output's own rounding, or for fp16 products and bf16 output an eighth of it.  (One part there: 33 x 16K
-//     e4m3 52.9 us, 53.5 with two; 2 x 256K 82.5 and 82.4; 12 heads a KV head 40.6 and 45.)
+//     as large as the output's own rounding.  Only for an e4m3 cache with bf16 output is one part enough: fp16 products, an
+//     eighth of the output's rounding (two parts there, of which the products' power slows the clock: 2 x 256K 92 us, 86 with
+//     one; 33 x 16K 59.4 and 56.5; the output's distance from the 64-bit result 1% less).
 //     Where V may hold infinities (16-bit caches) the first part is rounded towards zero and the second kept above zero, so
 //     that both products of a weight and an infinity have its sign, as the weight's own has: a remainder of 0 or below 0 would
 //     make a NaN of it.
@@ -48,8 +49,8 @@
 //
 // Measured (calls in a row; of the measured 6.54 TB/s): 64 x up to 8192 tokens of 32/8 heads, bf16, 1.11 GB, 165 us (100%
 // and more: reads alone pass a copy's rate); 1 x 131072, 0.54 GB, 84 us (98%); 2 x up to 262144 of 28/4 heads, e4m3, 0.53 GB,
-// 88 us (92%; 82 at the clocks of a short run), 52% of the issue slots; 33 x up to 16001 of 28/4 heads, e4m3, 0.31 GB, 57.5 us
-// (81%; 53 at the clocks of a short run): 3 us from the launch to the first full stream (lengths, table, rows: three loads in
+// 86 us (94%; 82 at the clocks of a short run), 49% of the issue slots; 33 x up to 16001 of 28/4 heads, e4m3, 0.31 GB, 56.5 us
+// (83%; 53 at the clocks of a short run): 3 us from the launch to the first full stream (lengths, table, rows: three loads in
 // turn), 3 us between the first CTA that ends and the last, 4 us for the join.  1 x 500 of 32/8 heads, 2 MB, 4.5 us: the launch
 // 0.9, the same loads in turn and the warps' sums 1.8, the cluster's barrier and sums 1.8.
 #include <cfloat>
@@ -94,8 +95,7 @@ struct DecodeArgs {
 };
 
 // 16 bytes of the cache (`bytes` of them, then zeros) to shared memory.  Cached rows pass through L2 once: evicted first, they
-// leave it to the tables, lengths and partial sums (28/4 heads, 33 x up to 16001 tokens of e4m3, one part of each weight: 57 us
-// without, 53 with).
+// leave it to the tables, lengths and partial sums (28/4 heads, 33 x up to 16001 tokens of e4m3: 57 us without, 53 with).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   uint64_t policy;
   asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
@@ -191,6 +191,7 @@ struct DecodeWarp {
   static constexpr int kRowBytes = kDecTileBytes / TT;
   static constexpr int kChunks = kRowBytes / 16;  // 16-byte pieces of a row
   static constexpr uint32_t kFull = TT == 32 ? 0xFFFFFFFFu : 0xFFFFu;
+  static constexpr bool kSplitP = !(kE4m3 && DT<T>::is_bf16);    // P as two parts
   static constexpr float kShift = DT<MT>::is_bf16 ? 0.f : 15.f;  // log2 of the factor of P and l
   static constexpr float kLarge = 4096.f;                        // e4m3: scores beyond are weighed by weigh_large
   // V scales as the running maximum takes them: P is kept finite beyond, and the sum of 2^31 weights below.
@@ -567,10 +568,10 @@ struct DecodeWarp {
             split_weights<MT>(p[0], p[1], hi, lo);
           } else {
             hi = DT<MT>::pack(p[0], p[1]);
-            lo = DT<MT>::pack(p[0] - DT<MT>::lo(hi), p[1] - DT<MT>::hi(hi));
+            if constexpr (kSplitP) lo = DT<MT>::pack(p[0] - DT<MT>::lo(hi), p[1] - DT<MT>::hi(hi));
           }
           pb[n][i][h] = transpose8x8(hi);
-          pl[n][i][h] = transpose8x8(lo);
+          if constexpr (kSplitP) pl[n][i][h] = transpose8x8(lo);
         }
       }
 #pragma unroll
@@ -582,7 +583,7 @@ struct DecodeWarp {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           mma16816<MT>(o[n][i], a[0], a[1], a[2], a[3], pb[n][0][0], pb[n][0][1]);
-          mma16816<MT>(o[n][i], a[0], a[1], a[2], a[3], pl[n][0][0], pl[n][0][1]);
+          if constexpr (kSplitP) mma16816<MT>(o[n][i], a[0], a[1], a[2], a[3], pl[n][0][0], pl[n][0][1]);
         }
       } else {
         // transposed pairs of codes: {token 2t: channels 2g, 2g+1; token 2t+1: channels 2g, 2g+1}; channel 2g becomes
@@ -596,7 +597,7 @@ struct DecodeWarp {
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma16816<MT>(o[n][i], a0, a1, a2, a3, pb[n][k][0], pb[n][k][1]);
-            mma16816<MT>(o[n][i], a0, a1, a2, a3, pl[n][k][0], pl[n][k][1]);
+            if constexpr (kSplitP) mma16816<MT>(o[n][i], a0, a1, a2, a3, pl[n][k][0], pl[n][k][1]);
           }
         }
       }

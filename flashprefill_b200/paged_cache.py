@@ -85,7 +85,8 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 
     A sequence of length 0 gives zeros and -inf, as does one whose length is outside [0, P * page_size].  Infinite values of a
     16-bit cache keep to the softmax (any weight makes the channel infinite; a weight that vanishes, below 2^-39 of the largest
-    for float16 and 2^-100 for bfloat16, makes it NaN, as 0 times infinity).  ``sm_scale`` is 1/sqrt(128) by default.  ``workspace``: uint8 of at least ``paged_decode_workspace_bytes``, taken from the caching
+    for float16 and 2^-100 for bfloat16, makes it NaN, as 0 times infinity).  Weights meet the values with 16 bits or more; with 11,
+    an eighth of the output's rounding, where an e4m3 cache is answered in bfloat16.  ``sm_scale`` is 1/sqrt(128) by default.  ``workspace``: uint8 of at least ``paged_decode_workspace_bytes``, taken from the caching
     allocator by default; calls that may overlap on the GPU (other streams, graphs replayed side by side) need one each.
     Results do not depend on the order in which the GPU runs its blocks: the same call gives the same bits (the same sequences
     behind a table of another width may be split, and rounded, in another way)."""
