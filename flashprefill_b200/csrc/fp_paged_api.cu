@@ -115,7 +115,7 @@ void head_groups(int G, int* ngroups, int* nh) {
 // 10.6 us with 8 x 4 warps an item, 7.7 with 8 x 12; 1 x 500, one tile a warp either way, 4.5 and 6.0).
 // Else pieces of the line of all units.  Clusters win up to there (1 x 8192 tokens 10.6 us, 13.0 in pieces; 256 x up to 600 of
 // 8/2 heads 18.3 and 21.4; 64 x up to 1024, 16 tiles, 27.6 and 28.2) and lose beyond (32 x up to 2100, 33 tiles, 41 us and 29.3
-// in pieces; 8 x up to 32000 of 48/4 heads, e4m3, 60 and 44).  Few items, each of several pieces, take wide CTAs, which leave a
+// in pieces; 8 x up to 32000 of 48/4 heads, e4m3 to bf16, 54 and 41).  Few items, each of several pieces, take wide CTAs, which leave a
 // third as many partial sums (2 x up to 262144 tokens of 28/4 heads, e4m3: 81.6 us, narrow 82.5); many ragged ones narrow CTAs,
 // which wait for one another less (64 x up to 8192 of 32/8: 168 us, wide 172).
 constexpr int kSms = 148;
