@@ -49,10 +49,10 @@
 //
 // Measured (calls in a row; of the measured 6.54 TB/s): 64 x up to 8192 tokens of 32/8 heads, bf16, 1.11 GB, 165 to 170 us (100%
 // and more: reads alone pass a copy's rate); 1 x 131072, 0.54 GB, 84 us (98%); 2 x up to 262144 of 28/4 heads, e4m3, 0.53 GB,
-// 86 to 88 us (92 to 94%; 82 at the clocks of a short run), 52% of the issue slots; 33 x up to 16001 of 28/4 heads, e4m3, 0.31 GB, 56.5 us
-// (83%; 53 at the clocks of a short run): 3 us from the launch to the first full stream (lengths, table, rows: three loads in
-// turn), 3 us between the first CTA that ends and the last, 4 us for the join.  1 x 500 of 32/8 heads, 2 MB, 4.5 us: the launch
-// 0.9, the same loads in turn and the warps' sums 1.8, the cluster's barrier and sums 1.8.
+// 86 to 88 us (92 to 94%; 82 at the clocks of a short run), 52% of the issue slots; 33 x up to 16001 of 28/4 heads, e4m3, 0.31
+// GB, 56.8 us (82%; 53 at the clocks of a short run): 3 us from the launch to the first full stream (lengths, table, rows: three
+// loads in turn), 3 us between the first CTA that ends and the last, 4 us for the join.  1 x 500 of 32/8 heads, 2 MB, 4.5 us: the
+// launch 0.9, the same loads in turn and the warps' sums 1.8, the cluster's barrier and sums 1.8.
 #include <cfloat>
 #include <type_traits>
 
